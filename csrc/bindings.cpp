@@ -41,6 +41,19 @@ int64_t fp8_sf_bytes(int64_t rows, int64_t k);
 void grouped_gemm_fp8(int64_t mode, torch::Tensor a, torch::Tensor sfa, torch::Tensor b, torch::Tensor sfb,
                       torch::Tensor out, c10::optional<torch::Tensor> pre, torch::Tensor probs, torch::Tensor total,
                       int64_t n_probs, int64_t b_rows, double gmax, double lo, double hi, torch::Tensor err);
+// fp4_kv.cu
+void fp4_kv_write(torch::Tensor k, torch::Tensor v, torch::Tensor pages, torch::Tensor slots, torch::Tensor err);
+void fp4_kv_read(torch::Tensor pages, torch::Tensor slots, torch::Tensor k, torch::Tensor v, torch::Tensor err);
+torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tensor table, torch::Tensor lengths,
+                               int64_t window, c10::optional<torch::Tensor> sink, double softcap, double scale,
+                               torch::Tensor err);
+// pages.cu
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> fork_pages(torch::Tensor pool, torch::Tensor table,
+                                                                   torch::Tensor lengths, torch::Tensor refcount,
+                                                                   torch::Tensor parents, torch::Tensor children,
+                                                                   int64_t page_rows, torch::Tensor err);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> compact_pages(torch::Tensor pool, torch::Tensor table,
+                                                                      torch::Tensor refcount, torch::Tensor err);
 // decode_attn.cu
 void decode_attention(torch::Tensor q, torch::Tensor k_win, torch::Tensor v_win, torch::Tensor pos,
                       c10::optional<torch::Tensor> sink_sw, double softcap, int64_t mode,
@@ -189,6 +202,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("compress_pool_bwd", &sv4::compress_pool_bwd);
   m.def("fp8_quant_blocks", &sv4::fp8_quant_blocks);
   m.def("gemm_fp8", &sv4::gemm_fp8);
+  m.def("fp4_kv_write", &sv4::fp4_kv_write);
+  m.def("fp4_kv_read", &sv4::fp4_kv_read);
+  m.def("fp4_kv_attention", &sv4::fp4_kv_attention);
+  m.def("fork_pages", &sv4::fork_pages);
+  m.def("compact_pages", &sv4::compact_pages);
   m.def("decode_attention", &sv4::decode_attention);
   m.def("decode_attention_paged", &sv4::decode_attention_paged);
   m.def("decode_window_split", &sv4::decode_window_split);

@@ -24,6 +24,7 @@ enum ErrorCode : int {
   kErrPeerTimeout = 5,      // cross-GPU flag never arrived
   kErrBounds = 6,           // gathered / scattered index out of range (index_ok)
   kErrCapacity = 7,         // expert-parallel receive layout exceeded the buffer capacity
+  kErrPages = 8,            // a page pool had too few free pages for a fork
 };
 
 __device__ __forceinline__ void record_error(int* err, int code) {

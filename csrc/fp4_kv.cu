@@ -1,0 +1,439 @@
+// A paged K / V cache held in 4 bits (MXFP4): rows quantised into pages, rows read back, and
+// attention that reads the pages as they are.
+//
+// Page of R rows of one sequence, for each K / V head a slab of R * d * 17 / 16 bytes:
+//   K codes (R x d/2) | V codes (R x d/2) | K scales (R x d/32) | V scales (R x d/32)
+// Byte j of a row's codes holds dim 2j (low four bits) and 2j + 1.  A code is E2M1 (sign, two
+// exponent bits, one mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6); 32 dims share the scale
+// 2^(byte - 127).  The scale's exponent is the smallest e with amax <= 6 * 2^e, at least -126;
+// byte 255 marks a block that held a NaN or an infinity and reads as NaN.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace sv4 {
+namespace {
+
+constexpr int kBlock = 32;  // values that share a scale
+
+template <typename T>
+__device__ __forceinline__ float as_float(T v);
+template <>
+__device__ __forceinline__ float as_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float as_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float as_float<__half>(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half(v); }
+
+// Eight values in one or two 16-byte accesses.
+template <typename T>
+struct alignas(16) Eight {
+  T v[8];
+};
+
+// 2^(byte - 127); 255 is NaN.  Byte 0 (2^-127 in E8M0) is never written and reads as 0.
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
+}
+
+__device__ __forceinline__ float e2m1_value(uint32_t code) {
+  const uint32_t two = (code >> 1) & 3u, m = code & 1u;
+  const float mag = two == 0 ? 0.5f * m : __uint_as_float(((two + 126u) << 23) | (m << 22));
+  return (code & 8u) ? -mag : mag;
+}
+
+// Nearest E2M1 magnitude of a >= 0 (in units of the scale), a tie going to the smaller one.
+__device__ __forceinline__ uint32_t e2m1_code(float a) {
+  return (a > 0.25f) + (a > 0.75f) + (a > 1.25f) + (a > 1.75f) + (a > 2.5f) + (a > 3.5f) + (a > 5.0f);
+}
+
+struct RowsArgs {
+  const void* src[2];     // write: K, V rows
+  void* dst[2];           // read: K, V rows
+  int64_t row_stride[2];  // elements
+  int64_t head_stride[2];
+  uint8_t* pages;
+  int64_t page_stride;
+  const int64_t* slots;
+  int64_t rows, n_slots;  // n_slots: pages * R
+  int heads, R, slab;
+  int* err;
+};
+
+// Thread = eight values of one row; four neighbouring threads share a scale.
+template <typename T, int D>
+__global__ void fp4_kv_write_kernel(const RowsArgs a) {
+  constexpr int kPer = D / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int part = static_cast<int>(i % kPer);
+  const int64_t unit = i / kPer;
+  const int kv = static_cast<int>(unit & 1);
+  const int head = static_cast<int>((unit >> 1) % a.heads);
+  const int64_t row = (unit >> 1) / a.heads;
+  const int64_t slot = row < a.rows ? a.slots[row] : -1;
+  // rows that are skipped keep their lanes for the shuffles
+  const bool live = slot != -1 && row < a.rows && index_ok(slot, 0, a.n_slots, a.err);
+  Eight<T> x;
+  float f[8];
+  float amax = 0.f;
+  if (live) {
+    x = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(a.src[kv]) + row * a.row_stride[kv] +
+                                           head * a.head_stride[kv] + part * 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[j] = as_float<T>(x.v[j]);
+      const float m = fabsf(f[j]);
+      amax = m <= 3.402823466e38f ? fmaxf(amax, m) : INFINITY;  // a NaN must not be dropped by fmaxf
+      if (isinf(amax)) break;
+    }
+  }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  if (!live) return;
+  const uint32_t bits = __float_as_uint(amax);
+  // amax = 1.m * 2^x: the exponent is x - 2 while 1.m <= 1.5
+  const int e = max(-126, static_cast<int>(bits >> 23) - 129 + ((bits & 0x7fffffu) > 0x400000u ? 1 : 0));
+  const bool bad = isinf(amax);
+  const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  uint32_t word = 0;
+  if (!bad) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t c = e2m1_code(fabsf(f[j]) * inv);
+      word |= (c | (f[j] < 0.f && c != 0 ? 8u : 0u)) << (4 * j);
+    }
+  }
+  const int64_t page = slot / a.R;
+  const int r = static_cast<int>(slot % a.R);
+  uint8_t* slab = a.pages + page * a.page_stride + static_cast<int64_t>(head) * a.slab;
+  *reinterpret_cast<uint32_t*>(slab + (kv * a.R + r) * (D / 2) + part * 4) = word;
+  if ((part & 3) == 0) slab[a.R * D + (kv * a.R + r) * (D / 32) + part / 4] = static_cast<uint8_t>(bad ? 255 : e + 127);
+}
+
+template <typename T, int D>
+__global__ void fp4_kv_read_kernel(const RowsArgs a) {
+  constexpr int kPer = D / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int part = static_cast<int>(i % kPer);
+  const int64_t unit = i / kPer;
+  const int kv = static_cast<int>(unit & 1);
+  const int head = static_cast<int>((unit >> 1) % a.heads);
+  const int64_t row = (unit >> 1) / a.heads;
+  if (row >= a.rows) return;
+  const int64_t slot = a.slots[row];
+  Eight<T> y;
+  uint32_t word = 0;
+  float s = 0.f;
+  if (slot != -1 && index_ok(slot, 0, a.n_slots, a.err)) {
+    const int r = static_cast<int>(slot % a.R);
+    const uint8_t* slab = a.pages + slot / a.R * a.page_stride + static_cast<int64_t>(head) * a.slab;
+    word = *reinterpret_cast<const uint32_t*>(slab + (kv * a.R + r) * (D / 2) + part * 4);
+    s = scale_of(slab[a.R * D + (kv * a.R + r) * (D / 32) + part / 4]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y.v[j] = from_float<T>(e2m1_value((word >> (4 * j)) & 15u) * s);
+  *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.dst[kv]) + ((row * a.heads + head) * D + part * 8)) = y;
+}
+
+// ------------------------------------------------------------------------------ attention
+struct AttnArgs {
+  const void* q;
+  int64_t q_b, q_h, q_t;  // strides in elements
+  const uint8_t* pages;
+  int64_t page_stride, n_pages;
+  const int* table;
+  const int* lengths;
+  const float* sink;
+  void* out;  // (B, H, T, d) contiguous
+  int B, H, Hk, T, P, R, slab, window;
+  float scale, softcap;
+  int* err;
+};
+
+constexpr int kThreads = 128;
+
+// out[b, h, t] = sum_j p_j v_j / (sum_j p_j + exp(sink_h - m)), p_j = exp(s_j - m), over the keys
+// max(0, pos - window + 1) .. pos, pos = length - T + t; a row without a key gives zero.
+// One block per (token, head, sequence): thread = key for the scores, thread = dim for the sums,
+// with the running maximum and sum of a one-pass softmax over tiles of 128 keys.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) fp4_kv_attn_kernel(const AttnArgs a) {
+  __shared__ float qs[D];
+  __shared__ float ps[kThreads];
+  __shared__ float red[kThreads / 32];
+  const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z, i = threadIdx.x;
+  const int head = h / (a.H / a.Hk);
+  const T* q = static_cast<const T*>(a.q) + b * a.q_b + h * a.q_h + t * a.q_t;
+  for (int d = i; d < D; d += kThreads) qs[d] = as_float<T>(q[d]);
+  const int64_t cap = static_cast<int64_t>(a.P) * a.R;
+  int64_t len = max(0, a.lengths[b]);
+  if (len > cap) {
+    record_error(a.err, kErrBounds);
+    len = cap;
+  }
+  const int64_t end = len - a.T + t + 1;  // one past the last visible key
+  const int64_t begin = a.window > 0 ? max(static_cast<int64_t>(0), end - a.window) : 0;
+  const int* table = a.table + static_cast<int64_t>(b) * a.P;
+  const int64_t half = static_cast<int64_t>(a.R) * D / 2;
+  float m = a.sink != nullptr ? a.sink[h] : -INFINITY;
+  float l = a.sink != nullptr ? 1.f : 0.f;
+  float acc[D / kThreads > 0 ? D / kThreads : 1] = {0.f};
+  __syncthreads();
+  for (int64_t j0 = begin; j0 < end; j0 += kThreads) {
+    const int64_t j = j0 + i;
+    float s = -INFINITY;
+    if (j < end) {
+      const int page = table[j / a.R];
+      if (index_ok(page, 0, a.n_pages, a.err)) {
+        const int r = static_cast<int>(j % a.R);
+        const uint8_t* slab = a.pages + page * a.page_stride + static_cast<int64_t>(head) * a.slab;
+        float dot = 0.f;
+        for (int blk = 0; blk < D / kBlock; ++blk) {
+          float part = 0.f;
+          for (int c = 0; c < kBlock / 2; ++c) {
+            const uint32_t byte = slab[r * (D / 2) + blk * (kBlock / 2) + c];
+            part += qs[blk * kBlock + 2 * c] * e2m1_value(byte & 15u) + qs[blk * kBlock + 2 * c + 1] * e2m1_value(byte >> 4);
+          }
+          dot += part * scale_of(slab[2 * half + r * (D / 32) + blk]);
+        }
+        s = dot * a.scale;
+        if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
+      }
+    }
+    float mx = s;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, mx, o);
+      mx = isnan(other) ? other : fmaxf(mx, other);
+    }
+    if (i % 32 == 0) red[i / 32] = mx;
+    __syncthreads();
+    float next = m;
+    for (int w = 0; w < kThreads / 32; ++w) next = fmaxf(next, red[w]);
+    const float keep = m == -INFINITY ? 0.f : __expf(m - next);
+    const float p = s == -INFINITY ? 0.f : expf(s - next);
+    ps[i] = p;
+    m = next;
+    __syncthreads();
+    float sum = 0.f;
+    for (int k = 0; k < kThreads; ++k) sum += ps[k];
+    l = l * keep + sum;
+    if (i < D) {
+#pragma unroll
+      for (int x = 0; x < D / kThreads + (D < kThreads); ++x) acc[x] *= keep;
+      for (int k = 0; k < kThreads; ++k) {
+        const float pk = ps[k];
+        if (pk == 0.f) continue;
+        const int64_t jk = j0 + k;
+        const int r = static_cast<int>(jk % a.R);
+        const uint8_t* slab = a.pages + table[jk / a.R] * a.page_stride + static_cast<int64_t>(head) * a.slab;
+#pragma unroll
+        for (int x = 0; x < D / kThreads + (D < kThreads); ++x) {
+          const int d = i + x * kThreads;
+          const uint32_t byte = slab[half + r * (D / 2) + d / 2];
+          acc[x] += pk * e2m1_value((d & 1) ? byte >> 4 : byte & 15u) *
+                    scale_of(slab[2 * half + a.R * (D / 32) + r * (D / 32) + d / 32]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.H + h) * a.T + t) * D;
+  if (i < D)
+    for (int x = 0; x < D / kThreads + (D < kThreads); ++x)
+      out[i + x * kThreads] = from_float<T>(l > 0.f || isnan(l) ? acc[x] / l : 0.f);
+}
+
+// Numbers in messages go through std::to_string: the stream operators of the toolchain's
+// libstdc++ and torch's do not agree on the locale's number facets.
+std::string num(int64_t v) { return std::to_string(v); }
+
+// Checks of a pages tensor; returns the rows per page.
+int page_rows_of(const torch::Tensor& pages, int64_t d, const char* who) {
+  TORCH_CHECK(pages.is_cuda() && pages.scalar_type() == at::kByte && pages.dim() == 3, who,
+              ": pages must be a CUDA uint8 tensor (n_pages, kv_heads, slab)");
+  TORCH_CHECK(d == 32 || d == 64 || d == 128, who, ": head_dim must be 32, 64 or 128, got ", num(d));
+  const int64_t slab = pages.size(2), rows = slab * 16 / (17 * d);
+  TORCH_CHECK(rows > 0 && rows % 16 == 0 && rows * d * 17 / 16 == slab, who, ": a slab of ", num(slab),
+              " bytes is not a multiple of 16 rows of head_dim ", num(d));
+  TORCH_CHECK(rows <= 65536, who, ": at most 65536 rows per page");
+  TORCH_CHECK(pages.stride(2) == 1 && (pages.size(1) == 1 || pages.stride(1) == slab) &&
+                  (pages.size(0) <= 1 || (pages.stride(0) % 16 == 0 && pages.stride(0) >= pages.size(1) * slab)) &&
+                  reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0,
+              who, ": pages must be contiguous within a page, with pages on 16-byte boundaries");
+  return static_cast<int>(rows);
+}
+
+template <typename F>
+void by_dim(int64_t d, F&& f) {
+  if (d == 32) f(std::integral_constant<int, 32>{});
+  else if (d == 64) f(std::integral_constant<int, 64>{});
+  else f(std::integral_constant<int, 128>{});
+}
+
+// f(T, D) for the rows' type and head dim.
+template <typename F>
+void by_type(at::ScalarType t, F&& f) {
+  if (t == at::kFloat) f(float{});
+  else if (t == at::kHalf) f(__half{});
+  else f(__nv_bfloat16{});
+}
+
+// A tensor whose rows of eight values can be read in 16-byte pieces.
+torch::Tensor rows_aligned(const torch::Tensor& t) {
+  const int64_t w = 16 / t.element_size();
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) == 1 || t.stride(i) % w == 0);
+  return ok ? t : t.contiguous();
+}
+
+RowsArgs rows_args(const torch::Tensor& pages, const torch::Tensor& slots, int64_t d, const char* who) {
+  RowsArgs a{};
+  a.R = page_rows_of(pages, d, who);
+  TORCH_CHECK(slots.is_cuda() && slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
+                  slots.device() == pages.device(), who, ": slots must be a contiguous int64 vector on the pages' device");
+  a.pages = pages.data_ptr<uint8_t>();
+  a.page_stride = pages.size(0) > 1 ? pages.stride(0) : pages.size(1) * pages.size(2);
+  a.slots = slots.data_ptr<int64_t>();
+  a.rows = slots.size(0);
+  a.n_slots = pages.size(0) * a.R;
+  a.heads = static_cast<int>(pages.size(1));
+  a.slab = static_cast<int>(pages.size(2));
+  return a;
+}
+
+}  // namespace
+
+// Quantise rows k, v (N, kv_heads, d) into `pages` at slots (N) = page * R + row; -1 skips a row.
+void fp4_kv_write(torch::Tensor k, torch::Tensor v, torch::Tensor pages, torch::Tensor slots, torch::Tensor err) {
+  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && k.scalar_type() == v.scalar_type() && k.is_cuda() &&
+                  v.device() == k.device() && k.device() == pages.device(),
+              "fp4_kv_write: k and v must be (rows, kv_heads, head_dim) of one type on the pages' device");
+  TORCH_CHECK(k.scalar_type() == at::kFloat || k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16,
+              "fp4_kv_write: rows must be bf16, fp16 or fp32");
+  const int64_t d = k.size(2);
+  RowsArgs a = rows_args(pages, slots, d, "fp4_kv_write");
+  TORCH_CHECK(k.size(1) == a.heads && k.size(0) == a.rows, "fp4_kv_write: ", num(k.size(0)), " rows of ",
+              num(k.size(1)), " heads for ", num(a.rows), " slots and pages of ", num(a.heads), " heads");
+  if (a.rows == 0) return;
+  c10::cuda::CUDAGuard guard(k.device());
+  k = rows_aligned(k);
+  v = rows_aligned(v);
+  a.src[0] = k.data_ptr();
+  a.src[1] = v.data_ptr();
+  a.row_stride[0] = k.stride(0);
+  a.row_stride[1] = v.stride(0);
+  a.head_stride[0] = k.stride(1);
+  a.head_stride[1] = v.stride(1);
+  a.err = err.data_ptr<int>();
+  const int64_t threads = a.rows * a.heads * 2 * (d / 8);
+  const unsigned grid = static_cast<unsigned>((threads + 255) / 256);
+  auto stream = at::cuda::getCurrentCUDAStream();
+  by_dim(d, [&](auto dim) {
+    by_type(k.scalar_type(), [&](auto t) {
+      fp4_kv_write_kernel<decltype(t), decltype(dim)::value><<<grid, 256, 0, stream>>>(a);
+    });
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// The rows at `slots` as k, v (N, kv_heads, d); a slot of -1 gives zeros.
+void fp4_kv_read(torch::Tensor pages, torch::Tensor slots, torch::Tensor k, torch::Tensor v, torch::Tensor err) {
+  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && k.scalar_type() == v.scalar_type() && k.is_contiguous() &&
+                  v.is_contiguous() && k.device() == pages.device() && v.device() == pages.device(),
+              "fp4_kv_read: outputs must be contiguous (rows, kv_heads, head_dim) of one type on the pages' device");
+  TORCH_CHECK(k.scalar_type() == at::kFloat || k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16,
+              "fp4_kv_read: rows must be bf16, fp16 or fp32");
+  const int64_t d = k.size(2);
+  RowsArgs a = rows_args(pages, slots, d, "fp4_kv_read");
+  TORCH_CHECK(k.size(1) == a.heads && k.size(0) == a.rows, "fp4_kv_read: outputs do not match slots and pages");
+  if (a.rows == 0) return;
+  c10::cuda::CUDAGuard guard(k.device());
+  a.dst[0] = k.data_ptr();
+  a.dst[1] = v.data_ptr();
+  a.err = err.data_ptr<int>();
+  const int64_t threads = a.rows * a.heads * 2 * (d / 8);
+  const unsigned grid = static_cast<unsigned>((threads + 255) / 256);
+  auto stream = at::cuda::getCurrentCUDAStream();
+  by_dim(d, [&](auto dim) {
+    by_type(k.scalar_type(), [&](auto t) {
+      fp4_kv_read_kernel<decltype(t), decltype(dim)::value><<<grid, 256, 0, stream>>>(a);
+    });
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// q (B, H, T, d) bf16 / fp16; table (B, P) int32; lengths (B) int32, the T tokens included.
+torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tensor table, torch::Tensor lengths,
+                               int64_t window, c10::optional<torch::Tensor> sink, double softcap, double scale,
+                               torch::Tensor err) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf),
+              "fp4_kv_attention: q must be a CUDA (B, H, T, head_dim) tensor in bf16 or fp16");
+  const int64_t B = q.size(0), H = q.size(1), T = q.size(2), d = q.size(3);
+  AttnArgs a{};
+  a.R = page_rows_of(pages, d, "fp4_kv_attention");
+  const int64_t Hk = pages.size(1);
+  TORCH_CHECK(Hk > 0 && H % Hk == 0, "fp4_kv_attention: ", num(H), " query heads over ", num(Hk),
+              " K/V heads");
+  TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B && table.is_contiguous() &&
+                  table.device() == q.device() && pages.device() == q.device(),
+              "fp4_kv_attention: table must be a contiguous (B, pages) int32 tensor on q's device");
+  TORCH_CHECK(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == B &&
+                  lengths.is_contiguous() && lengths.device() == q.device(),
+              "fp4_kv_attention: lengths must be a contiguous int32 vector of ", num(B), " on q's device");
+  TORCH_CHECK(table.size(1) * a.R <= INT32_MAX && window >= 0 && window <= INT32_MAX && softcap >= 0,
+              "fp4_kv_attention: window and softcap must not be negative, a table at most 2^31 - 1 rows wide");
+  if (sink.has_value())
+    TORCH_CHECK(sink->scalar_type() == at::kFloat && sink->numel() == H && sink->is_contiguous() &&
+                    sink->device() == q.device(), "fp4_kv_attention: sink must be ", num(H), " contiguous fp32 values");
+  c10::cuda::CUDAGuard guard(q.device());
+  torch::Tensor out = torch::empty({B, H, T, d}, q.options());
+  if (out.numel() == 0) return out;
+  q = rows_aligned(q);
+  a.q = q.data_ptr();
+  a.q_b = q.stride(0);
+  a.q_h = q.stride(1);
+  a.q_t = q.stride(2);
+  a.pages = pages.data_ptr<uint8_t>();
+  a.page_stride = pages.size(0) > 1 ? pages.stride(0) : Hk * pages.size(2);
+  a.n_pages = pages.size(0);
+  a.table = table.data_ptr<int>();
+  a.lengths = lengths.data_ptr<int>();
+  a.sink = sink.has_value() ? sink->data_ptr<float>() : nullptr;
+  a.out = out.data_ptr();
+  a.B = static_cast<int>(B);
+  a.H = static_cast<int>(H);
+  a.Hk = static_cast<int>(Hk);
+  a.T = static_cast<int>(T);
+  a.P = static_cast<int>(table.size(1));
+  a.slab = static_cast<int>(pages.size(2));
+  a.window = static_cast<int>(window);
+  a.scale = static_cast<float>(scale);
+  a.softcap = static_cast<float>(softcap);
+  a.err = err.data_ptr<int>();
+  TORCH_CHECK(B <= 65535 && H <= 65535, "fp4_kv_attention: at most 65535 sequences and heads");
+  const dim3 grid(static_cast<unsigned>(T), static_cast<unsigned>(H), static_cast<unsigned>(B));
+  auto stream = at::cuda::getCurrentCUDAStream();
+  by_dim(d, [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    if (q.scalar_type() == at::kHalf) fp4_kv_attn_kernel<__half, D><<<grid, kThreads, 0, stream>>>(a);
+    else fp4_kv_attn_kernel<__nv_bfloat16, D><<<grid, kThreads, 0, stream>>>(a);
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+}  // namespace sv4

@@ -1,0 +1,304 @@
+// Page bookkeeping of a paged cache, on the device: sequences forked (full pages shared by
+// reference counts, a partial last page copied), freed, and the pool compacted.  The pool is
+// any tensor whose first dimension is the page: its bytes are only moved.
+//
+// State: table (S, P) int32 page ids, -1 behind a row's last page; lengths (S) rows;
+// refcount (n_pages) rows of the table that hold a page, 0 = free.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "common.cuh"
+
+namespace sv4 {
+namespace {
+
+constexpr int kPlan = 1024;  // threads of the planning block
+
+// Exclusive prefix sum of `v` over a block of kPlan threads; *total gets the block's sum.
+__device__ __forceinline__ int block_scan(int v, int* total) {
+  __shared__ int sums[kPlan / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the last call's sums have been read
+  if (lane == 31) sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int s = sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    sums[lane] = s;
+  }
+  __syncthreads();
+  *total = sums[kPlan / 32 - 1];
+  return x - v + (warp > 0 ? sums[warp - 1] : 0);
+}
+
+struct ForkArgs {
+  uint8_t* pool;
+  int64_t page_bytes;
+  const int* table;
+  const int* lengths;
+  const int* refcount;
+  const int* parents;
+  const int* children;
+  int* new_table;
+  int* new_lengths;
+  int* new_refcount;
+  int* fresh;  // (F + 1): the page that takes the copied tail of fork i, or -1; [F]: 1 if all fitted
+  int S, P, F, n_pages, R;
+  int* err;
+};
+
+// What fork i does: false if its rows are out of range (recorded by `err`, when given).
+__device__ __forceinline__ bool fork_rows(const ForkArgs& a, int i, int* err, int* parent, int* child, int* len) {
+  *parent = a.parents[i];
+  *child = a.children[i];
+  *len = 0;
+  if (!index_ok(*child, 0, a.S, err) || !index_ok(*parent, -1, a.S, err)) return false;
+  if (*parent >= 0) {
+    *len = a.lengths[*parent];
+    if (!index_ok(*len, 0, static_cast<int64_t>(a.P) * a.R + 1, err)) return false;
+  }
+  return true;
+}
+
+// Block 0 gives every fork that copies a tail the next free page in ascending order; the other
+// blocks copy the state that the forks then change.
+__global__ void __launch_bounds__(kPlan) fork_plan_kernel(const ForkArgs a) {
+  if (blockIdx.x > 0) {
+    const int64_t step = static_cast<int64_t>(gridDim.x - 1) * kPlan;
+    const int64_t first = static_cast<int64_t>(blockIdx.x - 1) * kPlan + threadIdx.x;
+    for (int64_t i = first; i < static_cast<int64_t>(a.S) * a.P; i += step) a.new_table[i] = a.table[i];
+    for (int64_t i = first; i < a.S; i += step) a.new_lengths[i] = a.lengths[i];
+    for (int64_t i = first; i < a.n_pages; i += step) a.new_refcount[i] = a.refcount[i];
+    return;
+  }
+  int need = 0;
+  for (int i0 = 0; i0 < a.F; i0 += kPlan) {
+    const int i = i0 + threadIdx.x;
+    int parent = -1, child = -1, len = 0, copies = 0, total;
+    if (i < a.F && fork_rows(a, i, a.err, &parent, &child, &len)) copies = parent != child && len % a.R != 0;
+    const int rank = need + block_scan(copies, &total);
+    if (i < a.F) a.fresh[i] = copies ? rank : -1;  // the rank now, the page below
+    need += total;
+  }
+  // the first `need` free pages go into the tail of `fresh`
+  int* found = a.fresh + a.F + 1;
+  int have = 0;
+  for (int p0 = 0; p0 < a.n_pages && have < need; p0 += kPlan) {
+    const int p = p0 + threadIdx.x;
+    int total;
+    const int is_free = p < a.n_pages && a.refcount[p] == 0;
+    const int rank = have + block_scan(is_free, &total);
+    if (is_free && rank < need) found[rank] = p;
+    have += total;
+  }
+  __syncthreads();
+  const bool fits = have >= need;
+  if (!fits) record_error(a.err, kErrPages);
+  for (int i = threadIdx.x; i < a.F; i += kPlan) {
+    const int rank = a.fresh[i];
+    a.fresh[i] = rank >= 0 && fits ? found[rank] : -1;
+  }
+  if (threadIdx.x == 0) a.fresh[a.F] = fits;
+}
+
+// Block (i, y): fork i.  Every block copies its part of the tail page; block y = 0 also rewrites
+// the child's row and counts the pages that it leaves and takes (sums of whole numbers: their
+// order does not matter).
+__global__ void __launch_bounds__(256) fork_apply_kernel(const ForkArgs a) {
+  if (a.fresh[a.F] == 0) return;  // too few free pages: nothing changes
+  const int i = blockIdx.x;
+  int parent, child, len;
+  if (!fork_rows(a, i, nullptr, &parent, &child, &len) || parent == child) return;
+  const int fresh = a.fresh[i];
+  const int tail = len / a.R;
+  const int* from = a.table + static_cast<int64_t>(max(parent, 0)) * a.P;
+  if (blockIdx.y == 0) {
+    const int* old = a.table + static_cast<int64_t>(child) * a.P;
+    int* row = a.new_table + static_cast<int64_t>(child) * a.P;
+    for (int c = threadIdx.x; c < a.P; c += blockDim.x) {
+      const int gone = old[c];
+      if (gone >= 0 && index_ok(gone, 0, a.n_pages, a.err)) atomicSub(a.new_refcount + gone, 1);
+      int page = parent >= 0 ? from[c] : -1;
+      if (fresh >= 0 && c == tail) page = fresh;
+      row[c] = page;
+      if (page >= 0 && index_ok(page, 0, a.n_pages, a.err)) atomicAdd(a.new_refcount + page, 1);
+    }
+    if (threadIdx.x == 0) a.new_lengths[child] = len;
+  }
+  if (fresh < 0) return;
+  const int source = from[tail];
+  if (!index_ok(source, 0, a.n_pages, a.err)) return;
+  const uint4* src = reinterpret_cast<const uint4*>(a.pool + source * a.page_bytes);
+  uint4* dst = reinterpret_cast<uint4*>(a.pool + fresh * a.page_bytes);
+  const int64_t n = a.page_bytes / 16;
+  for (int64_t x = static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x; x < n;
+       x += static_cast<int64_t>(gridDim.y) * blockDim.x)
+    dst[x] = src[x];
+}
+
+struct CompactArgs {
+  uint8_t* pool;
+  int64_t page_bytes;
+  const int* table;
+  const int* refcount;
+  int* new_table;
+  int* new_refcount;
+  int* live;   // scalar: pages in use
+  int* where;  // (n_pages): where a page's contents go; -1: free
+  int* moves;  // (2, n_pages): k-th hole below the live count, k-th live page from it on
+  int64_t entries;
+  int n_pages;
+  int* err;
+};
+
+__global__ void __launch_bounds__(kPlan) compact_plan_kernel(const CompactArgs a) {
+  int live = 0;
+  for (int p0 = 0; p0 < a.n_pages; p0 += kPlan) {
+    const int p = p0 + threadIdx.x;
+    live += __syncthreads_count(p < a.n_pages && a.refcount[p] > 0);
+  }
+  if (threadIdx.x == 0) *a.live = live;
+  int* hole = a.moves;
+  int* late = a.moves + a.n_pages;
+  int holes = 0, lates = 0;
+  for (int p0 = 0; p0 < a.n_pages; p0 += kPlan) {
+    const int p = p0 + threadIdx.x;
+    const bool in = p < a.n_pages, used = in && a.refcount[p] > 0;
+    int total;
+    const int h = block_scan(in && !used && p < live, &total) + holes;
+    holes += total;
+    const int t = block_scan(used && p >= live, &total) + lates;
+    lates += total;
+    if (in && !used && p < live) hole[h] = p;
+    if (used && p >= live) late[t] = p;
+    if (in) a.where[p] = used && p < live ? p : -1;
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < lates; k += kPlan) a.where[late[k]] = hole[k];
+}
+
+// Sources are at or behind the live count and targets before it, so the copies are independent.
+__global__ void __launch_bounds__(256) compact_apply_kernel(const CompactArgs a) {
+  const int live = *a.live;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  for (int64_t i = first; i < a.entries; i += step) {
+    const int p = a.table[i];
+    a.new_table[i] = p < 0 ? -1 : index_ok(p, 0, a.n_pages, a.err) ? a.where[p] : -1;
+  }
+  for (int64_t p = first; p < a.n_pages; p += step) {
+    const int to = a.where[p];
+    if (p >= live) a.new_refcount[p] = 0;
+    if (to >= 0) a.new_refcount[to] = a.refcount[p];
+  }
+  const int64_t n = a.page_bytes / 16;
+  for (int p = live + blockIdx.x; p < a.n_pages; p += gridDim.x) {
+    const int to = a.where[p];
+    if (to < 0) continue;
+    const uint4* src = reinterpret_cast<const uint4*>(a.pool + p * a.page_bytes);
+    uint4* dst = reinterpret_cast<uint4*>(a.pool + to * a.page_bytes);
+    for (int64_t x = threadIdx.x; x < n; x += blockDim.x) dst[x] = src[x];
+  }
+}
+
+// The pool as pages of bytes; returns the bytes of a page.
+int64_t check_pool(const torch::Tensor& pool, const torch::Tensor& table, const torch::Tensor& refcount, const char* who) {
+  TORCH_CHECK(pool.is_cuda() && pool.dim() >= 2 && pool.is_contiguous(), who,
+              ": pool must be a contiguous CUDA tensor (n_pages, ...)");
+  const int64_t bytes = pool.size(0) > 0 ? pool.numel() / pool.size(0) * pool.element_size() : 0;
+  TORCH_CHECK(bytes % 16 == 0 && reinterpret_cast<uintptr_t>(pool.data_ptr()) % 16 == 0, who,
+              ": pages must be multiples of 16 bytes on 16-byte boundaries, got ", std::to_string(bytes));
+  TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous() &&
+                  table.device() == pool.device(), who, ": table must be a contiguous (rows, pages) int32 tensor on the pool's device");
+  TORCH_CHECK(refcount.scalar_type() == at::kInt && refcount.dim() == 1 && refcount.is_contiguous() &&
+                  refcount.device() == pool.device() && refcount.size(0) == pool.size(0) && pool.size(0) < INT32_MAX, who,
+              ": refcount must be a contiguous int32 vector of one count per page");
+  return bytes;
+}
+
+}  // namespace
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> fork_pages(torch::Tensor pool, torch::Tensor table,
+                                                                   torch::Tensor lengths, torch::Tensor refcount,
+                                                                   torch::Tensor parents, torch::Tensor children,
+                                                                   int64_t page_rows, torch::Tensor err) {
+  ForkArgs a{};
+  a.page_bytes = check_pool(pool, table, refcount, "fork_pages");
+  const int64_t F = parents.numel();
+  auto vec = [&](const torch::Tensor& t, int64_t n) {
+    return t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.size(0) == n && t.device() == pool.device();
+  };
+  TORCH_CHECK(vec(lengths, table.size(0)), "fork_pages: lengths must be a contiguous int32 vector, one per table row");
+  TORCH_CHECK(vec(parents, F) && vec(children, F),
+              "fork_pages: parents and children must be contiguous int32 vectors of one length on the pool's device");
+  TORCH_CHECK(page_rows > 0 && table.size(1) * page_rows <= INT32_MAX, "fork_pages: page_rows must be positive");
+  c10::cuda::CUDAGuard guard(pool.device());
+  if (F == 0) return {table.clone(), lengths.clone(), refcount.clone()};
+  auto new_table = torch::empty_like(table), new_lengths = torch::empty_like(lengths), new_refs = torch::empty_like(refcount);
+  auto fresh = torch::empty({2 * F + 1}, table.options());
+  a.pool = static_cast<uint8_t*>(pool.data_ptr());
+  a.table = table.data_ptr<int>();
+  a.lengths = lengths.data_ptr<int>();
+  a.refcount = refcount.data_ptr<int>();
+  a.parents = parents.data_ptr<int>();
+  a.children = children.data_ptr<int>();
+  a.new_table = new_table.data_ptr<int>();
+  a.new_lengths = new_lengths.data_ptr<int>();
+  a.new_refcount = new_refs.data_ptr<int>();
+  a.fresh = fresh.data_ptr<int>();
+  a.S = static_cast<int>(table.size(0));
+  a.P = static_cast<int>(table.size(1));
+  a.F = static_cast<int>(F);
+  a.n_pages = static_cast<int>(pool.size(0));
+  a.R = static_cast<int>(page_rows);
+  a.err = err.data_ptr<int>();
+  const int64_t copied = std::max<int64_t>({table.numel(), lengths.numel(), refcount.numel()});
+  auto stream = at::cuda::getCurrentCUDAStream();
+  fork_plan_kernel<<<1 + static_cast<unsigned>(std::min<int64_t>(147, (copied + kPlan - 1) / kPlan)), kPlan, 0, stream>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(64, a.page_bytes / 16384));
+  fork_apply_kernel<<<dim3(static_cast<unsigned>(F), static_cast<unsigned>(parts)), 256, 0, stream>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {new_table, new_lengths, new_refs};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> compact_pages(torch::Tensor pool, torch::Tensor table,
+                                                                      torch::Tensor refcount, torch::Tensor err) {
+  CompactArgs a{};
+  a.page_bytes = check_pool(pool, table, refcount, "compact_pages");
+  c10::cuda::CUDAGuard guard(pool.device());
+  auto new_table = torch::empty_like(table), new_refs = torch::empty_like(refcount);
+  auto live = torch::empty({}, table.options());
+  if (pool.size(0) == 0) return {table.clone(), new_refs, live.zero_()};
+  auto work = torch::empty({3 * pool.size(0)}, table.options());
+  a.pool = static_cast<uint8_t*>(pool.data_ptr());
+  a.table = table.data_ptr<int>();
+  a.refcount = refcount.data_ptr<int>();
+  a.new_table = new_table.data_ptr<int>();
+  a.new_refcount = new_refs.data_ptr<int>();
+  a.live = live.data_ptr<int>();
+  a.where = work.data_ptr<int>();
+  a.moves = a.where + pool.size(0);
+  a.entries = table.numel();
+  a.n_pages = static_cast<int>(pool.size(0));
+  a.err = err.data_ptr<int>();
+  auto stream = at::cuda::getCurrentCUDAStream();
+  compact_plan_kernel<<<1, kPlan, 0, stream>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  compact_apply_kernel<<<148 * 4, 256, 0, stream>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {new_table, new_refs, live};
+}
+
+}  // namespace sv4

@@ -33,7 +33,8 @@ def error_word(device: torch.device) -> Tensor:
 
 ERROR_NAMES = {1: "timeout waiting for a TMA stage", 2: "timeout waiting for a free stage",
                3: "timeout waiting for a TMEM accumulator", 4: "bad shape", 5: "peer timeout",
-               6: "index out of bounds", 7: "expert-parallel receive capacity exceeded"}
+               6: "index out of bounds", 7: "expert-parallel receive capacity exceeded",
+               8: "no free page left in the pool"}
 
 
 def check_errors(device: torch.device | None = None) -> None:
