@@ -1,20 +1,11 @@
 // A paged K / V cache held in 4 bits (MXFP4): rows quantised into pages, rows read back, and
-// attention that reads the pages as they are.
-//
-// Page of R rows of one sequence, for each K / V head a slab of R * d * 17 / 16 bytes:
-//   K codes (R x d/2) | V codes (R x d/2) | K scales (R x d/32) | V scales (R x d/32)
-// Byte j of a row's codes holds dim 2j (low four bits) and 2j + 1.  A code is E2M1 (sign, two
-// exponent bits, one mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6); 32 dims share the scale
-// 2^(byte - 127).  The scale's exponent is the smallest e with amax <= 6 * 2^e, at least -126;
-// byte 255 marks a block that held a NaN or an infinity and reads as NaN.
+// attention that reads the pages as they are (fp4_attn.cu).  The page format: fp4_kv.cuh.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include "common.cuh"
+#include "fp4_kv.cuh"
 
 namespace sv4 {
 namespace {
@@ -148,115 +139,6 @@ __global__ void fp4_kv_read_kernel(const RowsArgs a) {
   *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.dst[kv]) + ((row * a.heads + head) * D + part * 8)) = y;
 }
 
-// ------------------------------------------------------------------------------ attention
-struct AttnArgs {
-  const void* q;
-  int64_t q_b, q_h, q_t;  // strides in elements
-  const uint8_t* pages;
-  int64_t page_stride, n_pages;
-  const int* table;
-  const int* lengths;
-  const float* sink;
-  void* out;  // (B, H, T, d) contiguous
-  int B, H, Hk, T, P, R, slab, window;
-  float scale, softcap;
-  int* err;
-};
-
-constexpr int kThreads = 128;
-
-// out[b, h, t] = sum_j p_j v_j / (sum_j p_j + exp(sink_h - m)), p_j = exp(s_j - m), over the keys
-// max(0, pos - window + 1) .. pos, pos = length - T + t; a row without a key gives zero.
-// One block per (token, head, sequence): thread = key for the scores, thread = dim for the sums,
-// with the running maximum and sum of a one-pass softmax over tiles of 128 keys.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) fp4_kv_attn_kernel(const AttnArgs a) {
-  __shared__ float qs[D];
-  __shared__ float ps[kThreads];
-  __shared__ float red[kThreads / 32];
-  const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z, i = threadIdx.x;
-  const int head = h / (a.H / a.Hk);
-  const T* q = static_cast<const T*>(a.q) + b * a.q_b + h * a.q_h + t * a.q_t;
-  for (int d = i; d < D; d += kThreads) qs[d] = as_float<T>(q[d]);
-  const int64_t cap = static_cast<int64_t>(a.P) * a.R;
-  int64_t len = max(0, a.lengths[b]);
-  if (len > cap) {
-    record_error(a.err, kErrBounds);
-    len = cap;
-  }
-  const int64_t end = len - a.T + t + 1;  // one past the last visible key
-  const int64_t begin = a.window > 0 ? max(static_cast<int64_t>(0), end - a.window) : 0;
-  const int* table = a.table + static_cast<int64_t>(b) * a.P;
-  const int64_t half = static_cast<int64_t>(a.R) * D / 2;
-  float m = a.sink != nullptr ? a.sink[h] : -INFINITY;
-  float l = a.sink != nullptr ? 1.f : 0.f;
-  float acc[D / kThreads > 0 ? D / kThreads : 1] = {0.f};
-  __syncthreads();
-  for (int64_t j0 = begin; j0 < end; j0 += kThreads) {
-    const int64_t j = j0 + i;
-    float s = -INFINITY;
-    if (j < end) {
-      const int page = table[j / a.R];
-      if (index_ok(page, 0, a.n_pages, a.err)) {
-        const int r = static_cast<int>(j % a.R);
-        const uint8_t* slab = a.pages + page * a.page_stride + static_cast<int64_t>(head) * a.slab;
-        float dot = 0.f;
-        for (int blk = 0; blk < D / kBlock; ++blk) {
-          float part = 0.f;
-          for (int c = 0; c < kBlock / 2; ++c) {
-            const uint32_t byte = slab[r * (D / 2) + blk * (kBlock / 2) + c];
-            part += qs[blk * kBlock + 2 * c] * e2m1_value(byte & 15u) + qs[blk * kBlock + 2 * c + 1] * e2m1_value(byte >> 4);
-          }
-          dot += part * scale_of(slab[2 * half + r * (D / 32) + blk]);
-        }
-        s = dot * a.scale;
-        if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
-      }
-    }
-    float mx = s;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float other = __shfl_xor_sync(0xffffffffu, mx, o);
-      mx = isnan(other) ? other : fmaxf(mx, other);
-    }
-    if (i % 32 == 0) red[i / 32] = mx;
-    __syncthreads();
-    float next = m;
-    for (int w = 0; w < kThreads / 32; ++w) next = fmaxf(next, red[w]);
-    const float keep = m == -INFINITY ? 0.f : __expf(m - next);
-    const float p = s == -INFINITY ? 0.f : expf(s - next);
-    ps[i] = p;
-    m = next;
-    __syncthreads();
-    float sum = 0.f;
-    for (int k = 0; k < kThreads; ++k) sum += ps[k];
-    l = l * keep + sum;
-    if (i < D) {
-#pragma unroll
-      for (int x = 0; x < D / kThreads + (D < kThreads); ++x) acc[x] *= keep;
-      for (int k = 0; k < kThreads; ++k) {
-        const float pk = ps[k];
-        if (pk == 0.f) continue;
-        const int64_t jk = j0 + k;
-        const int r = static_cast<int>(jk % a.R);
-        const uint8_t* slab = a.pages + table[jk / a.R] * a.page_stride + static_cast<int64_t>(head) * a.slab;
-#pragma unroll
-        for (int x = 0; x < D / kThreads + (D < kThreads); ++x) {
-          const int d = i + x * kThreads;
-          const uint32_t byte = slab[half + r * (D / 2) + d / 2];
-          acc[x] += pk * e2m1_value((d & 1) ? byte >> 4 : byte & 15u) *
-                    scale_of(slab[2 * half + a.R * (D / 32) + r * (D / 32) + d / 32]);
-        }
-      }
-    }
-    __syncthreads();
-  }
-  T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.H + h) * a.T + t) * D;
-  if (i < D)
-    for (int x = 0; x < D / kThreads + (D < kThreads); ++x)
-      out[i + x * kThreads] = from_float<T>(l > 0.f || isnan(l) ? acc[x] / l : 0.f);
-}
-
 // Numbers in messages go through std::to_string: the stream operators of the toolchain's
 // libstdc++ and torch's do not agree on the locale's number facets.
 std::string num(int64_t v) { return std::to_string(v); }
@@ -383,7 +265,7 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   TORCH_CHECK(q.is_cuda() && q.dim() == 4 && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf),
               "fp4_kv_attention: q must be a CUDA (B, H, T, head_dim) tensor in bf16 or fp16");
   const int64_t B = q.size(0), H = q.size(1), T = q.size(2), d = q.size(3);
-  AttnArgs a{};
+  Fp4AttnArgs a{};
   a.R = page_rows_of(pages, d, "fp4_kv_attention");
   const int64_t Hk = pages.size(1);
   TORCH_CHECK(Hk > 0 && H % Hk == 0, "fp4_kv_attention: ", num(H), " query heads over ", num(Hk),
@@ -394,8 +276,8 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   TORCH_CHECK(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == B &&
                   lengths.is_contiguous() && lengths.device() == q.device(),
               "fp4_kv_attention: lengths must be a contiguous int32 vector of ", num(B), " on q's device");
-  TORCH_CHECK(table.size(1) * a.R <= INT32_MAX && window >= 0 && window <= INT32_MAX && softcap >= 0,
-              "fp4_kv_attention: window and softcap must not be negative, a table at most 2^31 - 1 rows wide");
+  TORCH_CHECK(table.size(1) * a.R <= INT32_MAX - 1024 && window >= 0 && window <= INT32_MAX && softcap >= 0,
+              "fp4_kv_attention: window and softcap must not be negative, a table less than 2^31 - 1024 rows wide");
   if (sink.has_value())
     TORCH_CHECK(sink->scalar_type() == at::kFloat && sink->numel() == H && sink->is_contiguous() &&
                     sink->device() == q.device(), "fp4_kv_attention: sink must be ", num(H), " contiguous fp32 values");
@@ -424,14 +306,20 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   a.scale = static_cast<float>(scale);
   a.softcap = static_cast<float>(softcap);
   a.err = err.data_ptr<int>();
-  TORCH_CHECK(B <= 65535 && H <= 65535, "fp4_kv_attention: at most 65535 sequences and heads");
-  const dim3 grid(static_cast<unsigned>(T), static_cast<unsigned>(H), static_cast<unsigned>(B));
-  auto stream = at::cuda::getCurrentCUDAStream();
-  by_dim(d, [&](auto dim) {
-    constexpr int D = decltype(dim)::value;
-    if (q.scalar_type() == at::kHalf) fp4_kv_attn_kernel<__half, D><<<grid, kThreads, 0, stream>>>(a);
-    else fp4_kv_attn_kernel<__nv_bfloat16, D><<<grid, kThreads, 0, stream>>>(a);
-  });
+  TORCH_CHECK(B <= 65535 && H * T <= (1 << 26), "fp4_kv_attention: at most 65535 sequences and 2^26 query rows in each");
+  // Slices: enough blocks to fill the device (three of four warps on each SM) twice over, so that
+  // sequences of different lengths even out, of no less than 256 keys.
+  const int64_t groups = B * Hk * ((H / Hk * T + 15) / 16);
+  const int64_t keys = std::min<int64_t>(table.size(1) * a.R, window > 0 ? window + T + 15 : INT32_MAX);
+  a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((2 * 3 * 148 + groups - 1) / groups, keys / 256)));
+  torch::Tensor parts;
+  if (a.splits > 1) {
+    const int64_t n = B * H * T * a.splits;
+    parts = torch::empty({n * (d + 2)}, q.options().dtype(at::kFloat));
+    a.part_ml = reinterpret_cast<float2*>(parts.data_ptr<float>());
+    a.part_out = parts.data_ptr<float>() + 2 * n;
+  }
+  fp4_attn_rows(a, static_cast<int>(d), q.scalar_type() == at::kHalf, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return out;
 }
