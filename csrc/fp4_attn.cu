@@ -6,12 +6,13 @@
 // bytes per token and K / V head are the traffic, and what bounds the kernel next to it is the
 // work of turning codes into operands.  So:
 //
-// * A warp owns 16 query rows (the G = H / Hk heads of a K / V head, times T tokens) and walks
-//   over tiles of 32 keys on its own: copies four tiles ahead (cp.async), no block-wide waits.
-//   A block's four warps take turns over the tiles of one slice of the keys and join at its end;
-//   a long sequence is cut into slices over blocks, joined by a second small kernel.
-// * Products run on mma.sync m16n8k16 in fp16, fp32 sums: with one to sixteen rows per head a
-//   128-row tcgen05 tile would be 7/8 empty.  Codes become fp16 pairs with cvt.e2m1x2, exact.
+// * A warp owns 8 or 16 query rows (the G = H / Hk heads of a K / V head, times T tokens) and
+//   walks over tiles of 32 keys on its own: copies (cp.async) two tiles ahead, no block-wide waits.
+//   A block's four warps take turns over its tiles and join at their end.  Blocks take equal parts
+//   of the list of all tiles; what is cut between blocks is joined by a second small kernel.
+// * Products run on mma.sync m16n8k16 in fp16 with fp32 sums, keys (then dims) as the 16 rows and
+//   query rows as the 8 columns: with one to sixteen rows a 128-row tcgen05 tile would be 7/8
+//   empty.  Codes become fp16 pairs with cvt.e2m1x2, exact.
 // * K and V scales are powers of two, applied to the fp16 pairs: exact while the exponent is in
 //   [-14, 13].  A tile with scales outside takes other exponents for K (28 from its own largest
 //   down) and runs its V product once per window of 28 exponents, the sums moved from unit to
@@ -20,9 +21,11 @@
 //   falls below 2^-38 of the row's largest is lost).  p is held times 2^15: fp16's 11 bits for
 //   weights down to 2^-29 of the largest.
 // * Operand order: dims and keys may be summed in any order, so a thread's operands are chosen to
-//   lie together: 4 bytes of a block per key for K; for V the d/16 bytes of its d/8 output dims,
-//   two keys' nibbles merged into the bytes that cvt turns into a pair.
+//   lie together: d/4 dims of a key for K; for V the d/16 bytes of its d/8 output dims, two keys'
+//   nibbles merged into the bytes that cvt turns into a pair.
 #include "fp4_kv.cuh"
+
+#include <algorithm>
 
 #include "common.cuh"
 
@@ -31,21 +34,25 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kTile = 32;  // keys per warp step
+// What a segment costs a block beside its tiles (queries, first copies, join), in tiles.
+constexpr int kSegmentCost = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D>
+template <int D, int NT>
 struct Cfg {
-  static constexpr int kC = D / 32;           // scale blocks per row
+  static constexpr int kRows = 8 * NT;         // query rows of a segment
+  static constexpr int kC = D / 32;            // scale blocks per row
   static constexpr int kCode = kTile * D / 2;  // bytes of K (or V) codes per stage
   static constexpr int kScale = kTile * kC;
   static constexpr int kStage = 2 * kCode + 2 * kScale;
-  static constexpr int kStages = 4;
-  static constexpr int kKTable = kTile * kC * 4;    // K scales as fp16 pairs, (row, block)
-  static constexpr int kVStride = kTile + 4;        // V scales fp16, (block, row), rows in pairs
+  static constexpr int kStages = 3;
+  static constexpr int kKTable = kTile * kC * 4;  // K scales as fp16 pairs, (row, block)
+  static constexpr int kVStride = kTile + 4;      // V scales fp16, (block, row), rows in pairs
   static constexpr int kVTable = kC * kVStride * 2;
   static constexpr int kWarpBytes = (kStages * kStage + kKTable + kVTable + 15) / 16 * 16;
-  static constexpr int kJoin = kWarps * 16 * D * 4 + kWarps * 16 * 8;
-  static constexpr int kSmem = kWarps * kWarpBytes > kJoin ? kWarps * kWarpBytes : kJoin;
+  static constexpr int kJoin = kWarps * kRows * (D * 4 + 8);
+  static constexpr int kSmem = kWarps * kWarpBytes > kJoin ? kWarps * kWarpBytes : kJoin;  // the join reuses the rings
+  static constexpr int kBlocks = D == 128 && NT == 2 ? 3 : 4;  // per SM: 168 or 128 registers a thread
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -76,6 +83,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// 8 x 8 fp16 matrix, a row in four neighbouring lanes' pairs, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -87,11 +100,18 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return d;
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+// 2^(a - b) for a <= b, both possibly -inf
+__device__ __forceinline__ float shrink(float a, float b) { return a == b ? 1.f : ex2(a - b); }
 
 __device__ __forceinline__ float2 two_floats(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
 __device__ __forceinline__ float2 two_floats(uint32_t w, __nv_bfloat16) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Few {
+  T v[N];
+};
 
 // What the keys keep of the whole when a sink logit joins the denominator: their maximum is `top`
 // (log2 units) and their sum of p (times 2^15) is l.
@@ -101,20 +121,6 @@ __device__ __forceinline__ float share_beside(float sink, float top, float l) {
   if (s2 <= top) return l / (l + ex2(s2 - top + 15.f));
   const float mine = l * ex2(top - s2);
   return mine / (mine + 32768.f);
-}
-
-// Swizzled byte offset of 16-byte piece `piece` of row `row` in a tile of codes, such that what a
-// warp reads at once falls into different banks.
-template <int D>
-__device__ __forceinline__ int k_at(int row, int piece) {
-  constexpr int C = D / 32;
-  const int x = C == 4 ? (row >> 1) & 3 : C == 2 ? (row >> 2) & 1 : 0;
-  return row * (D / 2) + ((piece ^ x) << 4);
-}
-template <int D>
-__device__ __forceinline__ int v_at(int row, int piece) {
-  const int x = D == 128 ? (row & 2) : 0;
-  return row * (D / 2) + ((piece ^ x) << 4);
 }
 
 // Extremes of the scale bytes of the tile's rows (NaN blocks and zero blocks, bytes 0 and 1, left out).
@@ -139,524 +145,755 @@ __device__ __forceinline__ uint32_t scale_bits(int byte, int bias) {
 
 // The sums' unit moved from 2^from to 2^to: exact but for what leaves fp32's range at the small
 // end.  Towards smaller units only as far as the largest sum stays finite; returns the unit.
-template <int N>
-__device__ __forceinline__ int to_unit(float (&acc)[N][4], int from, int to) {
+template <int N, int NT>
+__device__ __forceinline__ int to_unit(float (&acc)[N][NT][4], int from, int to) {
   float big = 0.f;
 #pragma unroll
   for (int x = 0; x < N; ++x)
 #pragma unroll
-    for (int y = 0; y < 4; ++y) big = fmaxf(big, fabsf(acc[x][y]));
+    for (int z = 0; z < NT; ++z)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) big = fmaxf(big, fabsf(acc[x][z][y]));
   const int top = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23) - 127;
-  int up = max(-126, min(126, from - to));
-  up = min(up, max(0, 96 - top));
-  const float f = pow2f(up);
+  const int up = min(min(from - to, 126), max(0, 96 - top));
+  const float f = pow2f(max(up, -126)), again = pow2f(max(min(up + 126, 0), -126));
 #pragma unroll
   for (int x = 0; x < N; ++x)
 #pragma unroll
-    for (int y = 0; y < 4; ++y) acc[x][y] *= f;
+    for (int z = 0; z < NT; ++z)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) acc[x][z][y] = acc[x][z][y] * f * again;
   return from - up;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32, D == 128 ? 3 : 4) fp4_attn_rows_kernel(const Fp4AttnArgs a) {
-  using C = Cfg<D>;
+// The work as one list: for every sequence b, `row_tiles` (K / V head, 8 NT query rows) segments
+// of kSegmentCost + tiles(b) units each, the last tiles(b) of them key tiles.  Block i of the grid
+// takes the units [i per, (i + 1) per), so blocks have equal work whatever the lengths; a segment
+// whose tiles lie in several blocks is joined by the second kernel.  tiles(b) spans what any of
+// the T tokens may see.
+struct Span {
+  int len, start, tiles;  // sequence length, the tile boundary at or before the first key that anyone sees
+};
+
+__device__ __forceinline__ Span span_of(const Fp4AttnArgs& a, int b) {
+  Span s;
+  s.len = min(max(0, a.lengths[b]), a.P * a.R);
+  const int first = a.window > 0 ? max(0, s.len - a.T + 1 - a.window) : 0;
+  s.start = first & ~(a.R % kTile == 0 ? kTile - 1 : 15);
+  s.tiles = s.len > 0 ? (s.len - s.start + kTile - 1) / kTile : 0;
+  return s;
+}
+__device__ __forceinline__ int units_of(const Span& s) { return s.tiles > 0 ? s.tiles + kSegmentCost : 0; }
+
+// Sum of a segment's units for b < upto and over all b, by the whole block (every thread gets both).
+__device__ __forceinline__ void count_units(const Fp4AttnArgs& a, int upto, int64_t& before, int64_t& all) {
+  __shared__ int64_t part[2][32];
+  int64_t mine = 0, below = 0;
+  for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
+    const int n = units_of(span_of(a, b));
+    mine += n;
+    if (b < upto) below += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    below += __shfl_xor_sync(0xffffffffu, below, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    part[0][threadIdx.x >> 5] = below;
+    part[1][threadIdx.x >> 5] = mine;
+  }
+  __syncthreads();
+  before = all = 0;
+  for (int w = 0; w < static_cast<int>(blockDim.x + 31) / 32; ++w) {
+    before += part[0][w];
+    all += part[1][w];
+  }
+}
+
+// Units per block: at least one tile for each warp.
+__device__ __forceinline__ int64_t units_per_block(const Fp4AttnArgs& a, int64_t total) {
+  return max(static_cast<int64_t>(kWarps), (total + a.blocks - 1) / a.blocks);
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_rows_kernel(const Fp4AttnArgs a) {
+  using C = Cfg<D, NT>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int G = a.H / a.Hk;
-  const int tiles_per_head = (G * a.T + 15) / 16;
-  const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits, b = blockIdx.y;
-  const int head = tile / tiles_per_head, row0 = (tile % tiles_per_head) * 16;
-  const int rows = min(16, G * a.T - row0);
-
-  int len = max(0, a.lengths[b]);
-  const int cap = a.P * a.R;
-  if (len > cap) {
-    if (threadIdx.x == 0) record_error(a.err, kErrBounds);
-    len = cap;
-  }
-  // keys that row i (token t) may see: [lo, hi)
-  auto limits = [&](int i, int& lo, int& hi) {
-    const int t = (row0 + min(i, rows - 1)) / G;
-    hi = len - a.T + t + 1;
-    lo = a.window > 0 ? max(0, hi - a.window) : 0;
-  };
-  int lo0, hi0, lo1, hi1, first, last, inner_lo, inner_hi;
-  limits(g, lo0, hi0);
-  limits(g + 8, lo1, hi1);
-  limits(0, first, inner_hi);
-  limits(15, inner_lo, last);
-  last = max(last, 0);
-  const int start = first & ~15;
-  const int n_tiles = (last - start + kTile - 1) / kTile;  // 0 when no row has a key
-  const int per = (n_tiles + a.splits - 1) / a.splits;
-  const int t_begin = min(n_tiles, split * per), t_end = min(n_tiles, t_begin + per);
-  const int mine = t_end - t_begin > warp ? (t_end - t_begin - warp + kWarps - 1) / kWarps : 0;
-
-  // ---- q as the A operand: row g and g + 8, dims 32 b + 8 c .. + 7, scaled to fp16's top
-  uint32_t qf[C::kC][8];
-  float unit0, unit1;
-  {
-    const T* q = static_cast<const T*>(a.q) + b * a.q_b;
-    float unit[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = row0 + min(g + 8 * r, rows - 1);
-      const T* row = q + (head * G + i % G) * a.q_h + (i / G) * a.q_t;
-      uint4 raw[C::kC];
-      float amax = 0.f;
-#pragma unroll
-      for (int k = 0; k < C::kC; ++k) {
-        raw[k] = *reinterpret_cast<const uint4*>(row + 32 * k + 8 * c);
-        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float2 f = two_floats(w[x], T{});
-          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-      }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const int x = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-      const int up = amax > 0.f && x < 128 ? min(14 - x, 126) : 0;
-      const float f = pow2f(up);
-      unit[r] = pow2f(max(-up, -126));
-#pragma unroll
-      for (int k = 0; k < C::kC; ++k) {
-        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const float2 v = two_floats(w[y], T{});
-          // pair y: step y / 2, k half y % 2 -> A register 2 * (y % 2) + r
-          qf[k][(y >> 1) * 4 + (y & 1) * 2 + r] = pack_half2(v.x * f, v.y * f);
-        }
-      }
-    }
-    unit0 = unit[0];
-    unit1 = unit[1];
-  }
-  const float nat = a.softcap > 0.f ? a.scale : a.scale * kLog2e;  // softcap works on natural units
+  const int tiles_per_head = (G * a.T + C::kRows - 1) / C::kRows, row_tiles = a.Hk * tiles_per_head;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- per-warp ring of key tiles
   uint8_t* ring = smem + warp * C::kWarpBytes;
   uint32_t* ktab = reinterpret_cast<uint32_t*>(ring + C::kStages * C::kStage);
   __half* vtab = reinterpret_cast<__half*>(ring + C::kStages * C::kStage + C::kKTable);
   const uint32_t ring_u = smem_u32(ring);
-  const int* table = a.table + static_cast<int64_t>(b) * a.P;
 
-  // Where the halves (16 keys) of sixteen coming tiles lie: lane 2 i + h holds half h of tile i.
-  auto look_up = [&](int batch, const uint8_t*& at, int& in_page) {
-    const int i = batch * 16 + (lane >> 1);
-    const int key = start + (t_begin + warp + i * kWarps) * kTile + (lane & 1) * 16;
-    at = nullptr;
-    in_page = -1;
-    if (i < mine && key < last) {
-      const int slot = key / a.R;
-      const int page = table[slot];
-      if (index_ok(page, 0, a.n_pages, a.err)) {
-        at = a.pages + page * a.page_stride + static_cast<int64_t>(head) * a.slab;
-        in_page = key - slot * a.R;
-      }
+  const int scale_half = (lane / C::kC) & 1, scale_kv = lane / (2 * C::kC);
+  const int64_t scale_src = static_cast<int64_t>(a.R) * D + scale_kv * a.R * C::kC + lane % C::kC * 16;
+
+  // ---- this block's part of the list
+  int64_t ignored, total;
+  count_units(a, 0, ignored, total);
+  total *= row_tiles;
+  const int64_t per = units_per_block(a, total);
+  int64_t skip = blockIdx.x * per;  // into the sequences from b on
+  if (skip >= total) return;
+  int left = static_cast<int>(min(total - skip, per)), b = 0;
+  while (true) {      // 32 sequences at a time
+    const int64_t n = b + lane < a.B ? static_cast<int64_t>(units_of(span_of(a, b + lane))) * row_tiles : 0;
+    int64_t upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
     }
-  };
-  const uint8_t *at_now, *at_next;
-  int in_now, in_next;
-  look_up(0, at_now, in_now);
-  look_up(1, at_next, in_next);
-  uint32_t present = 0;  // two bits per stage: its halves that were copied
+    const uint32_t past = __ballot_sync(0xffffffffu, skip < upto);
+    if (past != 0) {
+      const int here = __ffs(past) - 1;
+      skip -= __shfl_sync(0xffffffffu, upto - n, here);
+      b += here;
+      break;
+    }
+    skip -= __shfl_sync(0xffffffffu, upto, 31);
+    b += 32;
+  }
+  Span sp = span_of(a, b);
+  int y = static_cast<int>(skip / units_of(sp)), from_unit = static_cast<int>(skip % units_of(sp));
+  // the scale's sign (or zero) goes into q; softcap works on natural units
+  const float nat = (a.scale != 0.f ? fabsf(a.scale) : 1.f) * (a.softcap > 0.f ? 1.f : kLog2e);
 
-  auto issue = [&](int i) {
-    if (i < mine) {
-      if ((i & 15) == 0 && i > 0) {
-        at_now = at_next;
-        in_now = in_next;
-        look_up((i >> 4) + 1, at_next, in_next);
-      }
-      const int stage = i % C::kStages;
-      const uint32_t dst = ring_u + stage * C::kStage;
-      present &= ~(3u << (2 * stage));
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int from = ((i & 15) << 1) | h;
-        const uint8_t* slab = reinterpret_cast<const uint8_t*>(
-            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at_now), from));
-        const int r = __shfl_sync(0xffffffffu, in_now, from);
-        if (slab == nullptr) continue;
-        present |= 1u << (2 * stage + h);
-        const uint8_t* k = slab + r * (D / 2);
-        const uint8_t* v = k + a.R * (D / 2);
-#pragma unroll
-        for (int x = lane; x < 16 * C::kC; x += 32) {  // 16 rows of kC pieces
-          const int row = h * 16 + x / C::kC, piece = x % C::kC;
-          copy16(dst + k_at<D>(row, piece), k + x * 16);
-          copy16(dst + C::kCode + v_at<D>(row, piece), v + x * 16);
+  while (true) {
+    const int units = min(left, units_of(sp) - from_unit);
+    const int from_tile = max(0, from_unit - kSegmentCost);
+    const int take = from_unit + units - kSegmentCost - from_tile;  // may be 0 or less: only the segment's cost
+    if (take > 0) {
+      const int head = y / tiles_per_head, row0 = (y % tiles_per_head) * C::kRows;
+      const int rows = min(C::kRows, G * a.T - row0);
+      // one past the last key that row i (token t) may see; rows behind the last repeat it
+      auto end_of = [&](int i) { return sp.len - a.T + (row0 + min(i, rows - 1)) / G + 1; };
+      const int last = end_of(C::kRows - 1), inner_hi = end_of(0);
+      const int first = a.window > 0 ? max(0, inner_hi - a.window) : 0, inner_lo = a.window > 0 ? max(0, last - a.window) : 0;
+      const int mine = take > warp ? (take - warp + kWarps - 1) / kWarps : 0;
+      const int base = sp.start + (from_tile + warp) * kTile;  // the warp's first key
+      const int* table = a.table + static_cast<int64_t>(b) * a.P;
+
+      // Where the halves (16 keys) of sixteen coming tiles lie: lane 2 i + h holds half h of tile i.
+      auto look_up = [&](int batch, const uint8_t*& slab, int& in_page) {
+        const int i = batch * 16 + (lane >> 1);
+        const int key = base + i * kWarps * kTile + (lane & 1) * 16;
+        slab = nullptr;
+        in_page = 0;
+        if (i < mine && key < last) {
+          const int slot = key / a.R;
+          const int page = table[slot];
+          if (index_ok(page, 0, a.n_pages, a.err)) {
+            slab = a.pages + page * a.page_stride + static_cast<int64_t>(head) * a.slab;
+            in_page = key - slot * a.R;
+          }
         }
-        // 16 rows of kC scale bytes: kC pieces for K and for V
-        if (lane < 2 * C::kC) {
-          const int kv = lane / C::kC, piece = lane % C::kC;
-          copy16(dst + 2 * C::kCode + kv * C::kScale + h * 16 * C::kC + piece * 16,
-                 slab + a.R * D + (kv * a.R + r) * C::kC + piece * 16);
+      };
+      const uint8_t *slab_now, *slab_next;
+      int in_now, in_next;
+      look_up(0, slab_now, in_now);
+      look_up(1, slab_next, in_next);
+      uint32_t present = 0;  // two bits per stage: its halves that were copied
+      int fill = 0, stage = 0;  // the next stages to copy into and to compute
+
+      auto issue = [&](int i) {
+        if (i >= mine) return;
+        if ((i & 15) == 0 && i > 0) {
+          slab_now = slab_next;
+          in_now = in_next;
+          look_up((i >> 4) + 1, slab_next, in_next);
         }
+        const int from = (i & 15) << 1;
+        const uint8_t* s0 = reinterpret_cast<const uint8_t*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(slab_now), from));
+        const int r0 = __shfl_sync(0xffffffffu, in_now, from);
+        const uint8_t* s1 = s0;
+        int r1 = r0 + 16;
+        if (a.R % kTile != 0) {  // else tiles start at multiples of 32 and lie in one page
+          s1 = reinterpret_cast<const uint8_t*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(slab_now), from + 1));
+          r1 = __shfl_sync(0xffffffffu, in_now, from + 1);
+        }
+        const uint32_t dst = ring_u + fill * C::kStage;
+        auto copy_codes = [&](const uint8_t* slab, int r, int to) {  // 16 rows of d/2 bytes
+          const uint8_t* k = slab + r * (D / 2) + lane * 16;
+          const uint8_t* v = k + a.R * (D / 2);
+          if (D >= 64 || lane < 16) {
+#pragma unroll
+            for (int x = 0; x < (D + 63) / 64; ++x) {
+              copy16(dst + to * (D / 2) + lane * 16 + x * 512, k + x * 512);
+              copy16(dst + C::kCode + to * (D / 2) + lane * 16 + x * 512, v + x * 512);
+            }
+          }
+        };
+        if (s0 != nullptr) copy_codes(s0, r0, 0);
+        if (s1 != nullptr) copy_codes(s1, r1, 16);
+        // scales: lane (K / V, half, 16-byte piece)
+        const uint8_t* sc = scale_half ? s1 : s0;
+        if (lane < 4 * C::kC && sc != nullptr)
+          copy16(dst + 2 * C::kCode + lane * 16, sc + scale_src + (scale_half ? r1 : r0) * C::kC);
+        present = (present & ~(3u << (2 * fill))) | (((s0 != nullptr ? 1u : 0u) | (s1 != nullptr ? 2u : 0u)) << (2 * fill));
+        fill = fill + 1 == C::kStages ? 0 : fill + 1;
+      };
+#pragma unroll
+      for (int i = 0; i < C::kStages - 1; ++i) {
+        issue(i);
+        copy_commit();
       }
-    }
-    copy_commit();
-  };
 
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  float acc[D / 8][4];
+      // ---- q as the B operand: row 8 z + g, dims c d/4 .. (c + 1) d/4, scaled to fp16's top
+      uint32_t qf[NT][C::kC][4];
+      float factor[NT][2];  // raw score -> softmax units, rows 8 z + 2 c + x
+      int hi[NT][2];        // one past the last visible key, for the same rows
 #pragma unroll
-  for (int x = 0; x < D / 8; ++x) acc[x][0] = acc[x][1] = acc[x][2] = acc[x][3] = 0.f;
-  int out_unit = 0;                  // acc holds sums times 2^-out_unit
-  float poison0 = 0.f, poison1 = 0.f;  // NaN once a visible V block was NaN
-
+      for (int z = 0; z < NT; ++z) {
+        const int i = row0 + min(8 * z + g, rows - 1);
+        const T* row = static_cast<const T*>(a.q) + b * a.q_b + (head * G + i % G) * a.q_h + (i / G) * a.q_t;
+        uint4 raw[C::kC];
+        float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < C::kStages - 1; ++i) issue(i);
-
-  for (int i = 0; i < mine; ++i) {
-    issue(i + C::kStages - 1);
-    copy_wait<C::kStages - 1>();
-    __syncwarp();
-    const int stage = i % C::kStages;
-    const uint8_t* buf = ring + stage * C::kStage;
-    const int key0 = start + (t_begin + warp + i * kWarps) * kTile;
-    const uint32_t halves = (present >> (2 * stage)) & 3u;
-
-    // ---- scales: lane = row
-    uint32_t kw = 0, vw = 0;
-    const int my_key = key0 + lane;
-    if (((halves >> (lane >> 4)) & 1u) && my_key >= first && my_key < last) {
-      if constexpr (C::kC == 4) {
-        kw = *reinterpret_cast<const uint32_t*>(buf + 2 * C::kCode + lane * 4);
-        vw = *reinterpret_cast<const uint32_t*>(buf + 2 * C::kCode + C::kScale + lane * 4);
-      } else if constexpr (C::kC == 2) {
-        kw = *reinterpret_cast<const uint16_t*>(buf + 2 * C::kCode + lane * 2);
-        vw = *reinterpret_cast<const uint16_t*>(buf + 2 * C::kCode + C::kScale + lane * 2);
-      } else {
-        kw = buf[2 * C::kCode + lane];
-        vw = buf[2 * C::kCode + C::kScale + lane];
-      }
-    }
-    int klo = 255, khi = 0, vlo = 255, vhi = 0;
-    bool knan = false, vnan = false;
-    scale_range(kw, C::kC, klo, khi, knan);
-    scale_range(vw, C::kC, vlo, vhi, vnan);
-    // exponents [-14, 13] are bytes 113 .. 140
-    const bool plain = __all_sync(0xffffffffu, min(klo, vlo) > 112 && max(khi, vhi) <= 140 && !knan && !vnan);
-    int kbias = 112, vbias = 112;
-    if (!plain) {
-      khi = __reduce_max_sync(0xffffffffu, khi);
-      vhi = __reduce_max_sync(0xffffffffu, vhi);
-      kbias = max(khi - 28, -14);
-      vbias = max(vhi - 28, 2);
-    }
-    {
-      uint32_t s[C::kC];
+        for (int k = 0; k < C::kC; ++k) {
+          raw[k] = *reinterpret_cast<const uint4*>(row + c * (D / 4) + 8 * k);
+          const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
 #pragma unroll
-      for (int x = 0; x < C::kC; ++x) {
-        const int byte = (kw >> (8 * x)) & 255;
-        s[x] = scale_bits(byte, kbias) * 0x10001u;
-        if (byte == 255) s[x] = 0x7e007e00u;
-      }
-      if constexpr (C::kC == 4) *reinterpret_cast<uint4*>(ktab + lane * 4) = make_uint4(s[0], s[1], s[2], s[3]);
-      else if constexpr (C::kC == 2) *reinterpret_cast<uint2*>(ktab + lane * 2) = make_uint2(s[0], s[1]);
-      else ktab[lane] = s[0];
-    }
-    const int pair_at = (lane & ~7) | ((lane & 3) * 2) | ((lane >> 2) & 1);  // keys c and c + 4 side by side
-    auto put_v_scales = [&](int bias) {
+          for (int x = 0; x < 4; ++x) {
+            const float2 f = two_floats(w[x], T{});
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int x = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+        const int up = amax > 0.f && x < 128 ? min(14 - x, 126) : 0;
+        const float f = a.scale > 0.f ? pow2f(up) : a.scale < 0.f ? -pow2f(up) : 0.f;
+        const float unit = pow2f(max(-up, -126)) * nat;
 #pragma unroll
-      for (int x = 0; x < C::kC; ++x)
-        vtab[x * C::kVStride + pair_at] = __ushort_as_half(static_cast<uint16_t>(scale_bits((vw >> (8 * x)) & 255, bias)));
-    };
-    put_v_scales(vbias);
-    __syncwarp();
-
-    // ---- scores: column n of key group j is key 8 j + n / 2 + 4 (n % 2)
-    float s[4][4];
-    const int k_row = (g >> 1) + 4 * (g & 1);
+        for (int k = 0; k < C::kC; ++k) {
+          const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-      const int row = 8 * j + k_row;
-      uint32_t sc[C::kC];
-      if constexpr (C::kC == 4) {
-        const uint4 t = *reinterpret_cast<const uint4*>(ktab + row * 4);
-        sc[0] = t.x; sc[1] = t.y; sc[2] = t.z; sc[3] = t.w;
-      } else if constexpr (C::kC == 2) {
-        const uint2 t = *reinterpret_cast<const uint2*>(ktab + row * 2);
-        sc[0] = t.x; sc[1] = t.y;
-      } else {
-        sc[0] = ktab[row];
-      }
+          for (int p = 0; p < 4; ++p) {
+            const float2 v = two_floats(w[p], T{});
+            qf[z][k][p] = pack_half2(v.x * f, v.y * f);
+          }
+        }
 #pragma unroll
-      for (int k = 0; k < C::kC; ++k) {
-        uint32_t h[4];
-        codes_to_half2(*reinterpret_cast<const uint32_t*>(buf + k_at<D>(row, k) + c * 4), h);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) h[y] = mul2(h[y], sc[k]);
-        mma16816(s[j], qf[k][0], qf[k][1], qf[k][2], qf[k][3], h[0], h[1]);
-        mma16816(s[j], qf[k][4], qf[k][5], qf[k][6], qf[k][7], h[2], h[3]);
-      }
-    }
-
-    // ---- softmax in units of log2
-    float f0 = unit0 * nat, f1 = unit1 * nat;
-    if (!plain) {
-      const float km = pow2f(max(kbias - 112, -126));
-      f0 *= km;
-      f1 *= km;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[j][0] *= f0;
-      s[j][1] *= f0;
-      s[j][2] *= f1;
-      s[j][3] *= f1;
-    }
-    if (a.softcap > 0.f) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[j][x] = a.softcap * kLog2e * tanhf(s[j][x] / a.softcap);
-    }
-    if (halves != 3u || key0 < inner_lo || key0 + kTile > inner_hi) {  // some row does not see some key
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int key = key0 + 8 * j + c + 4 * x;
-          const bool there = (halves >> (j >> 1)) & 1u;
-          if (!there || key < lo0 || key >= hi0) s[j][x] = -INFINITY;
-          if (!there || key < lo1 || key >= hi1) s[j][2 + x] = -INFINITY;
+        for (int n = 0; n < 2; ++n) {
+          factor[z][n] = __shfl_sync(0xffffffffu, unit, (2 * c + n) * 4);
+          hi[z][n] = end_of(8 * z + 2 * c + n);
         }
       }
-    }
-    float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
-      x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
-    }
-    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-    const bool moved = n0 != m0 || n1 != m1;
-    if (__any_sync(0xffffffffu, moved)) {
-      const float keep0 = n0 == m0 ? 1.f : ex2(m0 - n0), keep1 = n1 == m1 ? 1.f : ex2(m1 - n1);
-      l0 *= keep0;
-      l1 *= keep1;
-#pragma unroll
-      for (int x = 0; x < D / 8; ++x) {
-        acc[x][0] *= keep0;
-        acc[x][1] *= keep0;
-        acc[x][2] *= keep1;
-        acc[x][3] *= keep1;
-      }
-      m0 = n0;
-      m1 = n1;
-    }
-    // p times 2^15, a row without a key so far keeps p = 0
-    const float d0 = m0 == -INFINITY ? 0.f : 15.f - m0, d1 = m1 == -INFINITY ? 0.f : 15.f - m1;
-    uint32_t p[4][2];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        s[j][x] = ex2(s[j][x] + d0);
-        s[j][2 + x] = ex2(s[j][2 + x] + d1);
-      }
-      l0 += s[j][0] + s[j][1];
-      l1 += s[j][2] + s[j][3];
-      p[j][0] = pack_half2(s[j][0], s[j][1]);
-      p[j][1] = pack_half2(s[j][2], s[j][3]);
-    }
 
-    // ---- sums of p v: column n of dim group x is dim n d/8 + x
-    auto add_values = [&]() {
+      float m[NT][2], sums[NT][4];  // maximum and sum of p (elements 0, 1) of rows 8 z + 2 c + x
+      float acc[D / 16][NT][4];     // dims g d/8 + 2 x (elements 0, 1) and + 1 (2, 3), the same rows
+      float poison[NT][2];          // NaN once a visible V block of this thread's dims was NaN
+      int out_unit = 0;             // acc holds sums times 2^-out_unit
+      bool out_of_range = false;    // maxima above 2^16
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        constexpr int kWords = D >= 64 ? D / 64 : 1;
-        uint32_t w[4][kWords];  // keys c, c + 4, c + 8, c + 12 of the half
+      for (int z = 0; z < NT; ++z) {
+        m[z][0] = m[z][1] = -INFINITY;
+        poison[z][0] = poison[z][1] = 0.f;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int row = 16 * k + c + 4 * y;
-          if constexpr (D == 128) {
-            const uint2 t = *reinterpret_cast<const uint2*>(buf + C::kCode + v_at<D>(row, g >> 1) + (g & 1) * 8);
-            w[y][0] = t.x;
-            w[y][1] = t.y;
-          } else if constexpr (D == 64) {
-            w[y][0] = *reinterpret_cast<const uint32_t*>(buf + C::kCode + row * 32 + g * 4);
+        for (int p = 0; p < 4; ++p) sums[z][p] = 0.f;
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) acc[x][z][p] = 0.f;
+      }
+
+      for (int i = 0; i < mine; ++i) {
+        issue(i + C::kStages - 1);
+        copy_commit();  // an empty group too, so that the wait counts tiles
+        copy_wait<C::kStages - 1>();
+        __syncwarp();
+        const uint8_t* buf = ring + stage * C::kStage;
+        const int key0 = base + i * kWarps * kTile;
+        const uint32_t halves = (present >> (2 * stage)) & 3u;
+        stage = stage + 1 == C::kStages ? 0 : stage + 1;
+
+        // ---- scales: lane = row.  Exponents [-14, 13] are bytes 113 .. 140.
+        constexpr uint32_t kFill = 0x71717171u;  // an ordinary scale, for rows that nobody may see
+        uint32_t kw = kFill, vw = kFill;
+        const int my_key = key0 + lane;
+        if (((halves >> (lane >> 4)) & 1u) && my_key >= first && my_key < last) {
+          if constexpr (C::kC == 4) {
+            kw = *reinterpret_cast<const uint32_t*>(buf + 2 * C::kCode + lane * 4);
+            vw = *reinterpret_cast<const uint32_t*>(buf + 2 * C::kCode + C::kScale + lane * 4);
+          } else if constexpr (C::kC == 2) {
+            kw = *reinterpret_cast<const uint16_t*>(buf + 2 * C::kCode + lane * 2) | (kFill & 0xffff0000u);
+            vw = *reinterpret_cast<const uint16_t*>(buf + 2 * C::kCode + C::kScale + lane * 2) | (kFill & 0xffff0000u);
           } else {
-            w[y][0] = *reinterpret_cast<const uint16_t*>(buf + C::kCode + row * 16 + g * 2);
+            kw = buf[2 * C::kCode + lane] | (kFill & 0xffffff00u);
+            vw = buf[2 * C::kCode + C::kScale + lane] | (kFill & 0xffffff00u);
           }
         }
-        const __half* vs = vtab + (g * D / 256) * C::kVStride + 16 * k + 2 * c;
-        const uint32_t sa = *reinterpret_cast<const uint32_t*>(vs), sb = *reinterpret_cast<const uint32_t*>(vs + 8);
+        // All four bytes in [112, 140] at once: b + 16 and b + 19 both have 100 as their top bits.  (A
+        // byte that carries fails itself.)  112 would give the scale 0, so it is left to the careful way.
+        const uint32_t k16 = kw + 0x10101010u, v16 = vw + 0x10101010u;
+        const uint32_t odd = ((k16 ^ 0x80808080u) | ((k16 + 0x03030303u) ^ 0x80808080u) | (v16 ^ 0x80808080u) |
+                              ((v16 + 0x03030303u) ^ 0x80808080u)) & 0xe0e0e0e0u;
+        const uint32_t low = ((k16 - 0x01010101u) & (v16 - 0x01010101u) & 0x80808080u) ^ 0x80808080u;
+        bool plain = __all_sync(0xffffffffu, (odd | low) == 0);
+        int kbias = 112, vbias = 112;
+        uint32_t ks[4];
+        const int pair_at = (lane & ~7) | ((lane & 3) * 2) | ((lane >> 2) & 1);  // keys c and c + 4 side by side
+        auto put_v_scales = [&](int bias, int most) {  // of the blocks whose byte is `most` or less
 #pragma unroll
-        for (int z = 0; z < kWords; ++z) {
-          uint32_t even_a[4], odd_a[4], even_b[4], odd_b[4];
-          codes_to_half2((w[0][z] & 0x0f0f0f0fu) | ((w[1][z] << 4) & 0xf0f0f0f0u), even_a);
-          codes_to_half2(((w[0][z] >> 4) & 0x0f0f0f0fu) | (w[1][z] & 0xf0f0f0f0u), odd_a);
-          codes_to_half2((w[2][z] & 0x0f0f0f0fu) | ((w[3][z] << 4) & 0xf0f0f0f0u), even_b);
-          codes_to_half2(((w[2][z] >> 4) & 0x0f0f0f0fu) | (w[3][z] & 0xf0f0f0f0u), odd_b);
-#pragma unroll
-          for (int y = 0; y < (D >= 64 ? 4 : 2); ++y) {
-            mma16816(acc[8 * z + 2 * y], p[2 * k][0], p[2 * k][1], p[2 * k + 1][0], p[2 * k + 1][1],
-                     mul2(even_a[y], sa), mul2(even_b[y], sb));
-            mma16816(acc[8 * z + 2 * y + 1], p[2 * k][0], p[2 * k][1], p[2 * k + 1][0], p[2 * k + 1][1],
-                     mul2(odd_a[y], sa), mul2(odd_b[y], sb));
+          for (int x = 0; x < C::kC; ++x) {
+            const int byte = (vw >> (8 * x)) & 255;
+            vtab[x * C::kVStride + pair_at] = __ushort_as_half(static_cast<uint16_t>(byte <= most ? scale_bits(byte, bias) : 0));
           }
-        }
-      }
-    };
-    if (plain && out_unit == 0) {
-      add_values();
-    } else {
-      // windows of 28 exponents, the largest first, the sums in the unit of each
-      int bias = vbias;
-      while (true) {
-        const int got = out_unit = to_unit(acc, out_unit, bias - 112);
-        const bool limited = got != bias - 112;
-        if (limited || bias != vbias) {
-          __syncwarp();
-          put_v_scales(got + 112);
-          __syncwarp();
-        }
-        add_values();
-        if (plain || limited) break;
-        int next = 0;  // the largest byte that no window has held yet
+        };
+        bool vnan = false;
+        if (plain) {
+          const uint32_t kf = (k16 << 2) & 0x7c7c7c7cu, vf = (v16 << 2) & 0x7c7c7c7cu;  // fp16's high bytes
 #pragma unroll
-        for (int x = 0; x < C::kC; ++x) {
-          const int byte = (vw >> (8 * x)) & 255;
-          if (byte <= bias && byte > 1) next = max(next, byte);
+          for (int x = 0; x < C::kC; ++x) {
+            ks[x] = __byte_perm(kf, 0, 0x0404 | (x << 12) | (x << 4));
+            vtab[x * C::kVStride + pair_at] = __ushort_as_half(static_cast<uint16_t>(__byte_perm(vf, 0, 0x4404 | (x << 4))));
+          }
+        } else {
+          int klo = 255, khi = 0, vlo = 255, vhi = 0;
+          bool knan = false;
+          scale_range(kw, C::kC, klo, khi, knan);
+          scale_range(vw, C::kC, vlo, vhi, vnan);
+          plain = __all_sync(0xffffffffu, min(klo, vlo) > 112 && max(khi, vhi) <= 140 && !knan && !vnan);  // but for zero blocks
+          if (!plain) {
+            khi = __reduce_max_sync(0xffffffffu, khi);
+            vhi = __reduce_max_sync(0xffffffffu, vhi);
+            kbias = max(khi - 28, -14);
+            vbias = max(vhi - 28, 2);
+          }
+#pragma unroll
+          for (int x = 0; x < C::kC; ++x) {
+            const int byte = (kw >> (8 * x)) & 255;
+            ks[x] = byte == 255 ? 0x7e007e00u : scale_bits(byte, kbias) * 0x10001u;
+          }
+          put_v_scales(vbias, 254);
         }
-        next = __reduce_max_sync(0xffffffffu, next);
-        if (next == 0) break;
-        bias = next - 28;
-      }
-      if (__any_sync(0xffffffffu, vnan)) {
-        // a NaN block reaches the rows that see its key: this thread's sums lie in block c d/128
-        const int mine_block = c * D / 128;
-        for (int y = 0; y < kTile; ++y) {
-          const uint32_t word = __shfl_sync(0xffffffffu, vw, y);
-          if (((word >> (8 * mine_block)) & 255u) != 255u) continue;
-          const int key = key0 + y;
-          if (key >= lo0 && key < hi0) poison0 = NAN;
-          if (key >= lo1 && key < hi1) poison1 = NAN;
-        }
-      }
-    }
-    __syncwarp();  // the stage and the scale tables are free again
-  }
+        if constexpr (C::kC == 4) *reinterpret_cast<uint4*>(ktab + lane * 4) = make_uint4(ks[0], ks[1], ks[2], ks[3]);
+        else if constexpr (C::kC == 2) *reinterpret_cast<uint2*>(ktab + lane * 2) = make_uint2(ks[0], ks[1]);
+        else ktab[lane] = ks[0];
+        __syncwarp();
 
-  // ---- join the block's warps
+        // ---- scores: row n of key group j (8 keys) is key 8 j + n / 2 + 4 (n % 2)
+        const int k_row = (g >> 1) + 4 * (g & 1);
+        uint32_t kc[4][C::kC], ksc[4];
+        float s[2][NT][4];  // key groups 2 j (elements 0, 1) and 2 j + 1 (2, 3), rows 8 z + 2 c + x
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-  }
-  copy_wait<0>();
-  __syncthreads();  // all rings are free
-  float* sum = reinterpret_cast<float*>(smem);                            // (warp, row, dim)
-  float2* ml = reinterpret_cast<float2*>(smem + kWarps * 16 * D * 4);  // (warp, row)
-  if (c == 0) {
-    ml[warp * 16 + g] = make_float2(m0, l0);
-    ml[warp * 16 + g + 8] = make_float2(m1, l1);
-  }
-  __syncthreads();
-  // every part divided by the block's sum of p, so that no unit can overflow
-  float big[2] = {-INFINITY, -INFINITY}, part[2];
+        for (int j = 0; j < 4; ++j) {
+          const int row = 8 * j + k_row;
+          const uint8_t* from = buf + row * (D / 2) + c * (D / 8);
+          if constexpr (C::kC == 4) {
+            const uint4 t = *reinterpret_cast<const uint4*>(from);
+            kc[j][0] = t.x; kc[j][1] = t.y; kc[j][2] = t.z; kc[j][3] = t.w;
+          } else if constexpr (C::kC == 2) {
+            const uint2 t = *reinterpret_cast<const uint2*>(from);
+            kc[j][0] = t.x; kc[j][1] = t.y;
+          } else {
+            kc[j][0] = *reinterpret_cast<const uint32_t*>(from);
+          }
+          ksc[j] = ktab[row * C::kC + c * C::kC / 4];
+        }
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    float l = 0.f;
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) big[r] = fmaxf(big[r], ml[w * 16 + g + 8 * r].x);
+          for (int z = 0; z < NT; ++z) s[j][z][0] = s[j][z][1] = s[j][z][2] = s[j][z][3] = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 x = ml[w * 16 + g + 8 * r];
-      l += x.y * (x.x == big[r] ? 1.f : ex2(x.x - big[r]));
+        for (int k = 0; k < C::kC; ++k) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t ha[4], hb[4];
+            codes_to_half2(kc[2 * j][k], ha);
+            codes_to_half2(kc[2 * j + 1][k], hb);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              ha[p] = mul2(ha[p], ksc[2 * j]);
+              hb[p] = mul2(hb[p], ksc[2 * j + 1]);
+            }
+#pragma unroll
+            for (int z = 0; z < NT; ++z) {
+              mma16816(s[j][z], ha[0], hb[0], ha[1], hb[1], qf[z][k][0], qf[z][k][1]);
+              mma16816(s[j][z], ha[2], hb[2], ha[3], hb[3], qf[z][k][2], qf[z][k][3]);
+            }
+          }
+        }
+
+        // ---- softmax in units of log2: score s f
+        float f[NT][2];
+#pragma unroll
+        for (int z = 0; z < NT; ++z)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) f[z][n] = factor[z][n];
+        if (!plain) {
+          const float km = pow2f(kbias - 112);
+#pragma unroll
+          for (int z = 0; z < NT; ++z)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) f[z][n] = fmaxf(f[z][n] * km, 1.1754944e-38f);  // 0 would turn the mask's -inf into NaN
+        }
+        auto each_score = [&](auto&& change) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int z = 0; z < NT; ++z)
+#pragma unroll
+              for (int p = 0; p < 4; ++p) s[j][z][p] = change(s[j][z][p], j, z, p);
+        };
+        auto unit_factors = [&]() {
+#pragma unroll
+          for (int z = 0; z < NT; ++z) f[z][0] = f[z][1] = 1.f;
+        };
+        if (a.softcap > 0.f) {
+          each_score([&](float v, int, int z, int p) { return a.softcap * kLog2e * tanhf(v * f[z][p & 1] / a.softcap); });
+          unit_factors();
+        }
+        if (halves != 3u || key0 < inner_lo || key0 + kTile > inner_hi) {  // some row does not see some key
+          each_score([&](float v, int j, int z, int p) {
+            const int key = key0 + 16 * j + 8 * (p >> 1) + k_row, end = hi[z][p & 1];
+            const bool seen = ((halves >> j) & 1u) && key < end && (a.window == 0 || key >= end - a.window);
+            return seen ? v : -INFINITY;
+          });
+        }
+        float next[NT][2];
+        bool moved = false;
+        float most = 0.f;
+#pragma unroll
+        for (int z = 0; z < NT; ++z) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            float x = fmaxf(fmaxf(s[0][z][n], s[0][z][2 + n]), fmaxf(s[1][z][n], s[1][z][2 + n]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            next[z][n] = fmaxf(m[z][n], x * f[z][n]);
+            moved = moved || next[z][n] != m[z][n];
+            most = fmaxf(most, next[z][n] == -INFINITY ? 0.f : fabsf(next[z][n]));
+          }
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+          if (__any_sync(0xffffffffu, most > 65536.f)) out_of_range = true;
+#pragma unroll
+          for (int z = 0; z < NT; ++z) {
+            const float keep0 = shrink(m[z][0], next[z][0]), keep1 = shrink(m[z][1], next[z][1]);
+            sums[z][0] *= keep0;
+            sums[z][1] *= keep1;
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+              acc[x][z][0] *= keep0;
+              acc[x][z][1] *= keep1;
+              acc[x][z][2] *= keep0;
+              acc[x][z][3] *= keep1;
+            }
+            m[z][0] = next[z][0];
+            m[z][1] = next[z][1];
+          }
+        }
+        if (out_of_range) {
+          // the fused multiply-add below would keep the bits that rounding took from the maximum
+          each_score([&](float v, int, int z, int p) { return v * f[z][p & 1]; });
+          unit_factors();
+        }
+        // p times 2^15 (a row without a key so far keeps p = 0), as the B operand of the next product
+        uint32_t p[2][NT][2];
+#pragma unroll
+        for (int z = 0; z < NT; ++z) {
+          const float d0 = m[z][0] == -INFINITY ? 0.f : 15.f - m[z][0], d1 = m[z][1] == -INFINITY ? 0.f : 15.f - m[z][1];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              p[j][z][x] = transpose8(pack_half2(ex2(fmaf(s[j][z][2 * x], f[z][0], d0)), ex2(fmaf(s[j][z][2 * x + 1], f[z][1], d1))));
+          }
+          // the rounded weights' sums, as a product with ones
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            mma16816(sums[z], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, p[j][z][0], p[j][z][1]);
+        }
+
+        // ---- sums of p v: rows n and n + 8 of dim group x are dims n d/8 + 2 x and + 1
+        auto add_values = [&]() {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            constexpr int kWords = D >= 64 ? D / 64 : 1;
+            uint32_t w[4][kWords];  // keys c, c + 4, c + 8, c + 12 of the half
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const uint8_t* from = buf + C::kCode + (16 * j + c + 4 * x) * (D / 2) + g * (D / 16);
+              if constexpr (D == 128) {
+                const uint2 t = *reinterpret_cast<const uint2*>(from);
+                w[x][0] = t.x;
+                w[x][1] = t.y;
+              } else if constexpr (D == 64) {
+                w[x][0] = *reinterpret_cast<const uint32_t*>(from);
+              } else {
+                w[x][0] = *reinterpret_cast<const uint16_t*>(from);
+              }
+            }
+            const __half* vs = vtab + (g * D / 256) * C::kVStride + 16 * j + 2 * c;
+            const uint32_t sa = *reinterpret_cast<const uint32_t*>(vs), sb = *reinterpret_cast<const uint32_t*>(vs + 8);
+#pragma unroll
+            for (int k = 0; k < kWords; ++k) {
+              uint32_t even_a[4], odd_a[4], even_b[4], odd_b[4];
+              codes_to_half2((w[0][k] & 0x0f0f0f0fu) | ((w[1][k] << 4) & 0xf0f0f0f0u), even_a);
+              codes_to_half2(((w[0][k] >> 4) & 0x0f0f0f0fu) | (w[1][k] & 0xf0f0f0f0u), odd_a);
+              codes_to_half2((w[2][k] & 0x0f0f0f0fu) | ((w[3][k] << 4) & 0xf0f0f0f0u), even_b);
+              codes_to_half2(((w[2][k] >> 4) & 0x0f0f0f0fu) | (w[3][k] & 0xf0f0f0f0u), odd_b);
+#pragma unroll
+              for (int x = 0; x < (D >= 64 ? 4 : 2); ++x) {
+                const uint32_t a0 = mul2(even_a[x], sa), a1 = mul2(odd_a[x], sa), a2 = mul2(even_b[x], sb), a3 = mul2(odd_b[x], sb);
+#pragma unroll
+                for (int z = 0; z < NT; ++z) mma16816(acc[4 * k + x][z], a0, a1, a2, a3, p[j][z][0], p[j][z][1]);
+              }
+            }
+          }
+        };
+        if (plain && out_unit == 0) {
+          add_values();
+        } else {
+          // windows of 28 exponents, the largest first, the sums in the unit of each
+          int bias = vbias, most_byte = 254;
+          while (true) {
+            const int got = out_unit = to_unit(acc, out_unit, bias - 112);
+            const bool limited = got != bias - 112;
+            if (limited || bias != vbias) {
+              __syncwarp();
+              put_v_scales(got + 112, most_byte);
+              __syncwarp();
+            }
+            add_values();
+            if (plain || limited) break;
+            int below = 0;  // the largest byte that no window has held yet
+#pragma unroll
+            for (int x = 0; x < C::kC; ++x) {
+              const int byte = (vw >> (8 * x)) & 255;
+              if (byte <= bias && byte > 1) below = max(below, byte);
+            }
+            below = __reduce_max_sync(0xffffffffu, below);
+            if (below == 0) break;
+            most_byte = bias;
+            bias = below - 28;
+          }
+          if (__any_sync(0xffffffffu, vnan)) {
+            // a NaN block reaches the rows that see its key: this thread's dims lie in block g d/256
+            for (int x = 0; x < kTile; ++x) {
+              const uint32_t word = __shfl_sync(0xffffffffu, vw, x);
+              if (((word >> (8 * (g * D / 256))) & 255u) != 255u) continue;
+              const int key = key0 + x;
+#pragma unroll
+              for (int z = 0; z < NT; ++z)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+                  if (key < hi[z][n] && (a.window == 0 || key >= hi[z][n] - a.window)) poison[z][n] = NAN;
+            }
+          }
+        }
+        __syncwarp();  // the stage and the scale tables are free again
+      }
+
+      // ---- join the block's warps: every part divided by the block's sum of p, so that no unit can overflow
+      __syncthreads();  // all rings are free
+      float* sum = reinterpret_cast<float*>(smem);                                     // (warp, register, lane)
+      float2* ml = reinterpret_cast<float2*>(smem + kWarps * C::kRows * D * 4);  // (warp, row)
+      if (g == 0) {
+#pragma unroll
+        for (int z = 0; z < NT; ++z)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) ml[warp * C::kRows + 8 * z + 2 * c + n] = make_float2(m[z][n], sums[z][n]);
+      }
+      __syncthreads();
+      const float unit = pow2f(max(-126, min(126, out_unit)));
+      float top[NT][2], whole_l[NT][2];
+#pragma unroll
+      for (int z = 0; z < NT; ++z) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float2* part = ml + 8 * z + 2 * c + n;
+          top[z][n] = -INFINITY;
+          whole_l[z][n] = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) top[z][n] = fmaxf(top[z][n], part[w * C::kRows].x);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) whole_l[z][n] += part[w * C::kRows].y * shrink(part[w * C::kRows].x, top[z][n]);
+          const float share = whole_l[z][n] == 0.f ? 0.f : shrink(m[z][n], top[z][n]) / whole_l[z][n];
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+              sum[(((warp * (D / 16) + x) * NT + z) * 4 + 2 * p + n) * 32 + lane] = acc[x][z][2 * p + n] * share * unit + poison[z][n];
+        }
+      }
+      __syncthreads();
+      // This warp's part of the dim groups, of all warps' sums: the result if the whole segment is here,
+      // else part 0 (it began in an earlier block) or 1 (its first tile is here) of this block.
+      constexpr int kX = D >= 64 ? D / 64 : 1;
+      const bool whole = from_tile == 0 && take == sp.tiles;
+      const int64_t slot = (blockIdx.x * 2 + (from_tile == 0 ? 1 : 0)) * static_cast<int64_t>(C::kRows);
+      if (warp * kX < D / 16) {
+#pragma unroll
+        for (int z = 0; z < NT; ++z) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int i = 8 * z + 2 * c + n;
+            if (i >= rows) continue;
+            const int h = head * G + (row0 + i) % G, t = (row0 + i) / G;
+            const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.T + t;
+            const float keep = whole && a.sink != nullptr ? share_beside(a.sink[h], top[z][n], whole_l[z][n]) : 1.f;
+            Few<float, 2 * kX> o;
+#pragma unroll
+            for (int x = 0; x < kX; ++x) {
+#pragma unroll
+              for (int p = 0; p < 2; ++p) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w)
+                  v += sum[(((w * (D / 16) + warp * kX + x) * NT + z) * 4 + 2 * p + n) * 32 + lane];
+                o.v[2 * x + p] = v;
+              }
+            }
+            const int d = g * (D / 8) + 2 * warp * kX;
+            if (whole) {
+              Few<T, 2 * kX> r;
+#pragma unroll
+              for (int x = 0; x < 2 * kX; ++x) r.v[x] = static_cast<T>(o.v[x] * keep);
+              *reinterpret_cast<Few<T, 2 * kX>*>(static_cast<T*>(a.out) + row * D + d) = r;
+            } else {
+              *reinterpret_cast<Few<float, 2 * kX>*>(a.part_out + (slot + i) * D + d) = o;
+              if (warp == 0 && g == 0) a.part_ml[slot + i] = make_float2(top[z][n], whole_l[z][n]);
+            }
+          }
+        }
+      }
     }
-    const float m = r == 0 ? m0 : m1;
-    part[r] = l == 0.f ? 0.f : (m == big[r] ? 1.f : ex2(m - big[r])) / l;
-  }
-  const float unit = pow2f(max(-126, min(126, out_unit)));
-#pragma unroll
-  for (int x = 0; x < D / 8; ++x) {
-    float* row = sum + (warp * 16 + g) * D + x;
-    row[2 * c * (D / 8)] = acc[x][0] * part[0] * unit + poison0;
-    row[(2 * c + 1) * (D / 8)] = acc[x][1] * part[0] * unit + poison0;
-    row += 8 * D;
-    row[2 * c * (D / 8)] = acc[x][2] * part[1] * unit + poison1;
-    row[(2 * c + 1) * (D / 8)] = acc[x][3] * part[1] * unit + poison1;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * D; i += kWarps * 32) {
-    const int r = i / D, d = i % D;
-    float top = -INFINITY, l = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * 16 + r].x);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 x = ml[w * 16 + r];
-      l += x.y * (x.x == top ? 1.f : ex2(x.x - top));
-      o += sum[(w * 16 + r) * D + d];
+
+    // ---- the next segment
+    left -= units;
+    if (left == 0) return;
+    from_unit = 0;
+    if (++y == row_tiles) {
+      y = 0;
+      do sp = span_of(a, ++b);
+      while (sp.tiles == 0);
     }
-    const int h = head * G + (row0 + r) % G, t = (row0 + r) / G;
-    const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.T + t;
-    if (a.splits > 1) {
-      a.part_out[(at * a.splits + split) * D + d] = o;
-      if (d == 0) a.part_ml[at * a.splits + split] = make_float2(top, l);
-    } else {
-      if (a.sink != nullptr) o *= share_beside(a.sink[h], top, l);
-      static_cast<T*>(a.out)[at * D + d] = static_cast<T>(o);
-    }
+    __syncthreads();  // the join's sums have been read
   }
 }
 
-// Joins the slices of one row, in their order: thread = dim.
-template <typename T, int D>
-__global__ void __launch_bounds__(D) fp4_attn_join_kernel(const Fp4AttnArgs a) {
-  const int64_t row = blockIdx.x;
-  const int d = threadIdx.x;
-  const float2* ml = a.part_ml + row * a.splits;
-  float top = -INFINITY, l = 0.f, o = 0.f;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s].x);
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 x = ml[s];
-    if (x.y != 0.f) l += x.y * (x.x == top ? 1.f : ex2(x.x - top));
-  }
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 x = ml[s];
-    if (x.y == 0.f) continue;  // an empty slice
-    o += a.part_out[(row * a.splits + s) * D + d] * (x.y * (x.x == top ? 1.f : ex2(x.x - top)) / l);
-  }
-  if (a.sink != nullptr) o *= share_beside(a.sink[row / a.T % a.H], top, l);
-  static_cast<T*>(a.out)[row * D + d] = static_cast<T>(o);
-}
+// Joins the parts of one row of a segment, in their order; a segment that one block had whole is
+// done, one without keys is zero.  Warp = every eighth part, lane = D / 32 dims.
+constexpr int kJoinWarps = 8;
 
-template <typename T, int D>
-void launch(const Fp4AttnArgs& a, cudaStream_t stream) {
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kJoinWarps * 32) fp4_attn_join_kernel(const Fp4AttnArgs a) {
+  constexpr int kX = D / 32, kRows = Cfg<D, NT>::kRows;
+  __shared__ float sum[kJoinWarps][D];
+  __shared__ float2 ml[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.H / a.Hk;
-  const unsigned blocks = static_cast<unsigned>(a.Hk * ((G * a.T + 15) / 16) * a.splits);
-  cudaFuncSetAttribute(fp4_attn_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
-  fp4_attn_rows_kernel<T, D><<<dim3(blocks, a.B), kWarps * 32, Cfg<D>::kSmem, stream>>>(a);
-  if (a.splits > 1)
-    fp4_attn_join_kernel<T, D><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.H * a.T), D, 0, stream>>>(a);
+  const int tiles_per_head = (G * a.T + kRows - 1) / kRows, row_tiles = a.Hk * tiles_per_head;
+  const int in_tile = blockIdx.x % kRows, seg = blockIdx.x / kRows, b = seg / row_tiles, y = seg % row_tiles;
+  const int i = (y % tiles_per_head) * kRows + in_tile;  // query row of the head
+  const int h = y / tiles_per_head * G + i % G;
+
+  int64_t before, total;
+  count_units(a, b, before, total);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (i >= G * a.T) return;
+  T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.H + h) * a.T + i / G) * D;
+  if (threadIdx.x == 0 && a.lengths[b] > a.P * a.R) record_error(a.err, kErrBounds);
+  const Span sp = span_of(a, b);
+  if (sp.tiles == 0) {
+    for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) out[d] = static_cast<T>(0.f);
+    return;
+  }
+  const int64_t per = units_per_block(a, total * row_tiles);
+  const int64_t begin = before * row_tiles + static_cast<int64_t>(y) * units_of(sp) + kSegmentCost;  // its first tile
+  const int block0 = static_cast<int>(begin / per), block1 = static_cast<int>((begin + sp.tiles - 1) / per);
+  if (block0 == block1) return;
+
+  float top = -INFINITY, l = 0.f, o[kX] = {};
+  for (int x = block0 + warp; x <= block1; x += kJoinWarps) {
+    const int64_t slot = (static_cast<int64_t>(x) * 2 + (begin >= x * per ? 1 : 0)) * kRows + in_tile;
+    const float2 p = a.part_ml[slot];
+    const Few<float, kX> v = *reinterpret_cast<const Few<float, kX>*>(a.part_out + slot * D + lane * kX);
+    if (p.y == 0.f) continue;  // no key of this part is visible
+    const float next = fmaxf(top, p.x);
+    const float keep = l * shrink(top, next), add = p.y * shrink(p.x, next);
+    top = next;
+    l = keep + add;
+    const float old = keep / l, now = add / l;  // o is the mean so far
+#pragma unroll
+    for (int d = 0; d < kX; ++d) o[d] = o[d] * old + v.v[d] * now;
+  }
+#pragma unroll
+  for (int d = 0; d < kX; ++d) sum[warp][lane * kX + d] = o[d];
+  if (lane == 0) ml[warp] = make_float2(top, l);
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
+    float most = -INFINITY, all = 0.f, r = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) most = fmaxf(most, ml[w].x);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w)
+      if (ml[w].y != 0.f) all += ml[w].y * shrink(ml[w].x, most);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w)
+      if (ml[w].y != 0.f) r += sum[w][d] * (ml[w].y * shrink(ml[w].x, most) / all);
+    if (a.sink != nullptr) r *= share_beside(a.sink[h], most, all);
+    out[d] = static_cast<T>(r);
+  }
+}
+
+template <typename T, int D, int NT>
+void launch(Fp4AttnArgs& a, cudaStream_t stream) {
+  using C = Cfg<D, NT>;
+  const int64_t segments = fp4_attn_segments(a);
+  cudaFuncSetAttribute(fp4_attn_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  fp4_attn_rows_kernel<T, D, NT><<<a.blocks, kWarps * 32, C::kSmem, stream>>>(a);
+  // the join may start while the last blocks run: it waits where it reads their parts
+  cudaLaunchConfig_t join{};
+  join.gridDim = dim3(static_cast<unsigned>(segments * C::kRows));
+  join.blockDim = dim3(kJoinWarps * 32);
+  join.stream = stream;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  join.attrs = &early;
+  join.numAttrs = 1;
+  cudaLaunchKernelEx(&join, fp4_attn_join_kernel<T, D, NT>, static_cast<const Fp4AttnArgs&>(a));
+}
+
+template <typename T>
+void by_shape(Fp4AttnArgs& a, int d, cudaStream_t stream) {
+  const bool few = fp4_attn_rows_per_segment(a) == 8;
+  if (d == 32) few ? launch<T, 32, 1>(a, stream) : launch<T, 32, 2>(a, stream);
+  else if (d == 64) few ? launch<T, 64, 1>(a, stream) : launch<T, 64, 2>(a, stream);
+  else few ? launch<T, 128, 1>(a, stream) : launch<T, 128, 2>(a, stream);
 }
 
 }  // namespace
 
-void fp4_attn_rows(const Fp4AttnArgs& a, int d, bool half, cudaStream_t stream) {
-  if (half) {
-    if (d == 32) launch<__half, 32>(a, stream);
-    else if (d == 64) launch<__half, 64>(a, stream);
-    else launch<__half, 128>(a, stream);
-  } else {
-    if (d == 32) launch<__nv_bfloat16, 32>(a, stream);
-    else if (d == 64) launch<__nv_bfloat16, 64>(a, stream);
-    else launch<__nv_bfloat16, 128>(a, stream);
-  }
+int fp4_attn_rows_per_segment(const Fp4AttnArgs& a) { return a.H / a.Hk * a.T <= 8 ? 8 : 16; }
+
+int64_t fp4_attn_segments(const Fp4AttnArgs& a) {
+  const int rows = fp4_attn_rows_per_segment(a);
+  return static_cast<int64_t>(a.B) * a.Hk * ((static_cast<int64_t>(a.H / a.Hk) * a.T + rows - 1) / rows);
+}
+
+int fp4_attn_blocks(const Fp4AttnArgs& a, int d) {
+  const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.P) * a.R, a.window > 0 ? static_cast<int64_t>(a.window) + a.T + 31 : INT32_MAX);
+  const int64_t units = fp4_attn_segments(a) * ((keys + kTile - 1) / kTile + kSegmentCost);
+  const int64_t wave = 148 * (d == 128 && fp4_attn_rows_per_segment(a) == 16 ? 3 : 4);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wave, (units + kWarps - 1) / kWarps)));
+}
+
+void fp4_attn_rows(Fp4AttnArgs& a, int d, bool half, cudaStream_t stream) {
+  if (half) by_shape<__half>(a, d, stream);
+  else by_shape<__nv_bfloat16>(a, d, stream);
 }
 
 }  // namespace sv4

@@ -307,18 +307,12 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   a.softcap = static_cast<float>(softcap);
   a.err = err.data_ptr<int>();
   TORCH_CHECK(B <= 65535 && H * T <= (1 << 26), "fp4_kv_attention: at most 65535 sequences and 2^26 query rows in each");
-  // Slices: enough blocks to fill the device (three of four warps on each SM) twice over, so that
-  // sequences of different lengths even out, of no less than 256 keys.
-  const int64_t groups = B * Hk * ((H / Hk * T + 15) / 16);
-  const int64_t keys = std::min<int64_t>(table.size(1) * a.R, window > 0 ? window + T + 15 : INT32_MAX);
-  a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((2 * 3 * 148 + groups - 1) / groups, keys / 256)));
-  torch::Tensor parts;
-  if (a.splits > 1) {
-    const int64_t n = B * H * T * a.splits;
-    parts = torch::empty({n * (d + 2)}, q.options().dtype(at::kFloat));
-    a.part_ml = reinterpret_cast<float2*>(parts.data_ptr<float>());
-    a.part_out = parts.data_ptr<float>() + 2 * n;
-  }
+  TORCH_CHECK(fp4_attn_segments(a) * 16 < INT32_MAX, "fp4_kv_attention: too many query rows");
+  a.blocks = fp4_attn_blocks(a, static_cast<int>(d));
+  const int64_t part_rows = static_cast<int64_t>(a.blocks) * 2 * fp4_attn_rows_per_segment(a);
+  torch::Tensor parts = torch::empty({part_rows * (d + 2)}, q.options().dtype(at::kFloat));
+  a.part_ml = reinterpret_cast<float2*>(parts.data_ptr<float>());
+  a.part_out = parts.data_ptr<float>() + 2 * part_rows;
   fp4_attn_rows(a, static_cast<int>(d), q.scalar_type() == at::kHalf, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return out;

@@ -23,15 +23,21 @@ struct Fp4AttnArgs {
   const int* lengths;
   const float* sink;
   void* out;  // (B, H, T, d) contiguous
-  // split work: part s of row r = (b * H + h) * T + t is partial[r * splits + s]
-  float* part_out;  // (rows, splits, d): sum of p v, not divided
-  float2* part_ml;  // (rows, splits): maximum (log2 units), sum of p
-  int B, H, Hk, T, P, R, slab, window, splits;
+  // what is cut between blocks: block i has two parts of `rows` rows, (2 i + which) * rows ..
+  float* part_out;  // (blocks, 2, rows, d): mean of v under the part's own weights
+  float2* part_ml;  // (blocks, 2, rows): maximum score (log2 units), sum of p
+  int B, H, Hk, T, P, R, slab, window, blocks;
   float scale, softcap;
   int* err;
 };
 
+// Query rows (heads of a K / V head times tokens) of one unit of work, the number of those units
+// (sequence, K / V head, rows), and the blocks of one wave for head_dim d.
+int fp4_attn_rows_per_segment(const Fp4AttnArgs& a);
+int64_t fp4_attn_segments(const Fp4AttnArgs& a);
+int fp4_attn_blocks(const Fp4AttnArgs& a, int d);
+
 // Launch for head_dim d (32, 64, 128) and q in fp16 or bf16.
-void fp4_attn_rows(const Fp4AttnArgs& a, int d, bool half, cudaStream_t stream);
+void fp4_attn_rows(Fp4AttnArgs& a, int d, bool half, cudaStream_t stream);
 
 }  // namespace sv4
