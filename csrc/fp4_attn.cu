@@ -34,8 +34,9 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kTile = 32;  // keys per warp step
-// What a segment costs a block beside its tiles (queries, first copies, join), in tiles.
-constexpr int kSegmentCost = 8;
+// What a segment costs a block beside its tiles (queries, first copies, join), in tiles: with 8 blocks
+// that begin many short segments come last (prefill chunk 207 us, 176 with 16, 182 with 28).
+constexpr int kSegmentCost = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, int NT>
@@ -52,7 +53,9 @@ struct Cfg {
   static constexpr int kWarpBytes = (kStages * kStage + kKTable + kVTable + 15) / 16 * 16;
   static constexpr int kJoin = kWarps * kRows * (D * 4 + 8);
   static constexpr int kSmem = kWarps * kWarpBytes > kJoin ? kWarps * kWarpBytes : kJoin;  // the join reuses the rings
-  static constexpr int kBlocks = D == 128 && NT == 2 ? 3 : 4;  // per SM: 168 or 128 registers a thread
+  // Per SM.  16 rows: two blocks with all the registers they want beat three with spills (131072 keys of
+  // 8 heads and as many of another length: 99 and 110 us); 8 rows: four beat three (71 and 90 us).
+  static constexpr int kBlocks = D == 128 && NT == 2 ? 2 : 4;
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -71,6 +74,12 @@ __device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t (&o)[4]) {
       "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
       "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
       : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(w));
+}
+// The low four bits of every byte from a, the high ones from b.
+__device__ __forceinline__ uint32_t low_nibbles_of(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xca;" : "=r"(d) : "r"(0x0f0f0f0fu), "r"(a), "r"(b));  // mask ? a : b
+  return d;
 }
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -186,19 +195,16 @@ __device__ __forceinline__ Span span_of(const Fp4AttnArgs& a, int b) {
 __device__ __forceinline__ int units_of(const Span& s) { return s.tiles > 0 ? s.tiles + kSegmentCost : 0; }
 
 // Sum of a segment's units for b < upto and over all b, by the whole block (every thread gets both).
-__device__ __forceinline__ void count_units(const Fp4AttnArgs& a, int upto, int64_t& before, int64_t& all) {
-  __shared__ int64_t part[2][32];
-  int64_t mine = 0, below = 0;
+__device__ __forceinline__ void count_units(const Fp4AttnArgs& a, int upto, int& before, int& all) {
+  __shared__ int part[2][32];
+  int mine = 0, below = 0;
   for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
     const int n = units_of(span_of(a, b));
     mine += n;
     if (b < upto) below += n;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    below += __shfl_xor_sync(0xffffffffu, below, o);
-  }
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  below = __reduce_add_sync(0xffffffffu, below);
   if ((threadIdx.x & 31) == 0) {
     part[0][threadIdx.x >> 5] = below;
     part[1][threadIdx.x >> 5] = mine;
@@ -212,8 +218,8 @@ __device__ __forceinline__ void count_units(const Fp4AttnArgs& a, int upto, int6
 }
 
 // Units per block: at least one tile for each warp.
-__device__ __forceinline__ int64_t units_per_block(const Fp4AttnArgs& a, int64_t total) {
-  return max(static_cast<int64_t>(kWarps), (total + a.blocks - 1) / a.blocks);
+__device__ __forceinline__ int units_per_block(const Fp4AttnArgs& a, int total) {
+  return max(kWarps, static_cast<int>((static_cast<uint32_t>(total) + a.blocks - 1) / a.blocks));
 }
 
 template <typename T, int D, int NT>
@@ -235,19 +241,18 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
   const int64_t scale_src = static_cast<int64_t>(a.R) * D + scale_kv * a.R * C::kC + lane % C::kC * 16;
 
   // ---- this block's part of the list
-  int64_t ignored, total;
+  int ignored, total;
   count_units(a, 0, ignored, total);
   total *= row_tiles;
-  const int64_t per = units_per_block(a, total);
-  int64_t skip = blockIdx.x * per;  // into the sequences from b on
-  if (skip >= total) return;
-  int left = static_cast<int>(min(total - skip, per)), b = 0;
-  while (true) {      // 32 sequences at a time
-    const int64_t n = b + lane < a.B ? static_cast<int64_t>(units_of(span_of(a, b + lane))) * row_tiles : 0;
-    int64_t upto = n;
+  const int per = units_per_block(a, total);
+  if (static_cast<int64_t>(blockIdx.x) * per >= total) return;
+  int skip = blockIdx.x * per, left = min(total - skip, per), b = 0;  // skip: into the sequences from b on
+  while (true) {  // 32 sequences at a time
+    const int n = b + lane < a.B ? units_of(span_of(a, b + lane)) * row_tiles : 0;
+    int upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
     const uint32_t past = __ballot_sync(0xffffffffu, skip < upto);
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
     b += 32;
   }
   Span sp = span_of(a, b);
-  int y = static_cast<int>(skip / units_of(sp)), from_unit = static_cast<int>(skip % units_of(sp));
+  int y = skip / units_of(sp), from_unit = skip - y * units_of(sp);
   // the scale's sign (or zero) goes into q; softcap works on natural units
   const float nat = (a.scale != 0.f ? fabsf(a.scale) : 1.f) * (a.softcap > 0.f ? 1.f : kLog2e);
 
@@ -416,31 +421,32 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
         const uint32_t halves = (present >> (2 * stage)) & 3u;
         stage = stage + 1 == C::kStages ? 0 : stage + 1;
 
-        // ---- scales: lane = row.  Exponents [-14, 13] are bytes 113 .. 140.
-        constexpr uint32_t kFill = 0x71717171u;  // an ordinary scale, for rows that nobody may see
-        uint32_t kw = kFill, vw = kFill;
-        const int my_key = key0 + lane;
-        if (((halves >> (lane >> 4)) & 1u) && my_key >= first && my_key < last) {
-          if constexpr (C::kC == 4) {
-            kw = *reinterpret_cast<const uint32_t*>(buf + 2 * C::kCode + lane * 4);
-            vw = *reinterpret_cast<const uint32_t*>(buf + 2 * C::kCode + C::kScale + lane * 4);
-          } else if constexpr (C::kC == 2) {
-            kw = *reinterpret_cast<const uint16_t*>(buf + 2 * C::kCode + lane * 2) | (kFill & 0xffff0000u);
-            vw = *reinterpret_cast<const uint16_t*>(buf + 2 * C::kCode + C::kScale + lane * 2) | (kFill & 0xffff0000u);
-          } else {
-            kw = buf[2 * C::kCode + lane] | (kFill & 0xffffff00u);
-            vw = buf[2 * C::kCode + C::kScale + lane] | (kFill & 0xffffff00u);
-          }
+        // ---- scales, as fp16 pairs: of K for the rows 8 j + k_row and this thread's block c d/128, of V
+        // for the row pairs (16 j + c, + 4) and (+ 8, + 12) and its block g d/256.  Exponents
+        // [-14, 13] are bytes 113 .. 140; bytes of both are checked by lane = row.
+        const int k_row = (g >> 1) + 4 * (g & 1);
+        const uint8_t *kbytes = buf + 2 * C::kCode, *vbytes = kbytes + C::kScale;
+        uint32_t kw, vw;
+        if constexpr (C::kC == 4) {
+          kw = *reinterpret_cast<const uint32_t*>(kbytes + lane * 4);
+          vw = *reinterpret_cast<const uint32_t*>(vbytes + lane * 4);
+        } else if constexpr (C::kC == 2) {
+          kw = *reinterpret_cast<const uint16_t*>(kbytes + lane * 2) * 0x10001u;
+          vw = *reinterpret_cast<const uint16_t*>(vbytes + lane * 2) * 0x10001u;
+        } else {
+          kw = kbytes[lane] * 0x1010101u;
+          vw = vbytes[lane] * 0x1010101u;
         }
-        // All four bytes in [112, 140] at once: b + 16 and b + 19 both have 100 as their top bits.  (A
-        // byte that carries fails itself.)  112 would give the scale 0, so it is left to the careful way.
+        // All four bytes in [113, 140] at once: b + 16 and b + 19 both have 100 as their top bits, and
+        // b + 15 the highest.  (A byte that carries or borrows fails itself.)
         const uint32_t k16 = kw + 0x10101010u, v16 = vw + 0x10101010u;
         const uint32_t odd = ((k16 ^ 0x80808080u) | ((k16 + 0x03030303u) ^ 0x80808080u) | (v16 ^ 0x80808080u) |
                               ((v16 + 0x03030303u) ^ 0x80808080u)) & 0xe0e0e0e0u;
         const uint32_t low = ((k16 - 0x01010101u) & (v16 - 0x01010101u) & 0x80808080u) ^ 0x80808080u;
-        bool plain = __all_sync(0xffffffffu, (odd | low) == 0);
+        const bool inner = halves == 3u && key0 >= first && key0 + kTile <= last;  // every row was written
+        bool plain = true, vnan = false;
         int kbias = 112, vbias = 112;
-        uint32_t ks[4];
+        uint32_t ksc[4], vsc[2][2];
         const int pair_at = (lane & ~7) | ((lane & 3) * 2) | ((lane >> 2) & 1);  // keys c and c + 4 side by side
         auto put_v_scales = [&](int bias, int most) {  // of the blocks whose byte is `most` or less
 #pragma unroll
@@ -449,15 +455,28 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
             vtab[x * C::kVStride + pair_at] = __ushort_as_half(static_cast<uint16_t>(byte <= most ? scale_bits(byte, bias) : 0));
           }
         };
-        bool vnan = false;
-        if (plain) {
-          const uint32_t kf = (k16 << 2) & 0x7c7c7c7cu, vf = (v16 << 2) & 0x7c7c7c7cu;  // fp16's high bytes
+        auto get_v_scales = [&]() {
+          const __half* from = vtab + (g * D / 256) * C::kVStride + 2 * c;
 #pragma unroll
-          for (int x = 0; x < C::kC; ++x) {
-            ks[x] = __byte_perm(kf, 0, 0x0404 | (x << 12) | (x << 4));
-            vtab[x * C::kVStride + pair_at] = __ushort_as_half(static_cast<uint16_t>(__byte_perm(vf, 0, 0x4404 | (x << 4))));
-          }
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) vsc[j][x] = *reinterpret_cast<const uint32_t*>(from + 16 * j + 8 * x);
+        };
+        if (__all_sync(0xffffffffu, inner && (odd | low) == 0)) {
+          // (byte - 112) << 10 in one or both halves
+          constexpr uint32_t kOne = 0x0400u, kBoth = 0x04000400u;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ksc[j] = kbytes[(8 * j + k_row) * C::kC + c * C::kC / 4] * kBoth - 112u * kBoth;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint8_t* from = vbytes + (16 * j + 8 * x + c) * C::kC + g * D / 256;
+              vsc[j][x] = from[0] * kOne + (from[4 * C::kC] * (kOne << 16) - 112u * kBoth);
+            }
         } else {
+          const int my_key = key0 + lane;
+          if (!((halves >> (lane >> 4)) & 1u) || my_key < first || my_key >= last) kw = vw = 0x71717171u;  // nobody sees it
           int klo = 255, khi = 0, vlo = 255, vhi = 0;
           bool knan = false;
           scale_range(kw, C::kC, klo, khi, knan);
@@ -472,18 +491,17 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
 #pragma unroll
           for (int x = 0; x < C::kC; ++x) {
             const int byte = (kw >> (8 * x)) & 255;
-            ks[x] = byte == 255 ? 0x7e007e00u : scale_bits(byte, kbias) * 0x10001u;
+            ktab[lane * C::kC + x] = byte == 255 ? 0x7e007e00u : scale_bits(byte, kbias) * 0x10001u;
           }
           put_v_scales(vbias, 254);
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ksc[j] = ktab[(8 * j + k_row) * C::kC + c * C::kC / 4];
+          get_v_scales();
         }
-        if constexpr (C::kC == 4) *reinterpret_cast<uint4*>(ktab + lane * 4) = make_uint4(ks[0], ks[1], ks[2], ks[3]);
-        else if constexpr (C::kC == 2) *reinterpret_cast<uint2*>(ktab + lane * 2) = make_uint2(ks[0], ks[1]);
-        else ktab[lane] = ks[0];
-        __syncwarp();
 
         // ---- scores: row n of key group j (8 keys) is key 8 j + n / 2 + 4 (n % 2)
-        const int k_row = (g >> 1) + 4 * (g & 1);
-        uint32_t kc[4][C::kC], ksc[4];
+        uint32_t kc[4][C::kC];
         float s[2][NT][4];  // key groups 2 j (elements 0, 1) and 2 j + 1 (2, 3), rows 8 z + 2 c + x
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -498,7 +516,6 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           } else {
             kc[j][0] = *reinterpret_cast<const uint32_t*>(from);
           }
-          ksc[j] = ktab[row * C::kC + c * C::kC / 4];
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -550,7 +567,10 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           for (int z = 0; z < NT; ++z) f[z][0] = f[z][1] = 1.f;
         };
         if (a.softcap > 0.f) {
-          each_score([&](float v, int, int z, int p) { return a.softcap * kLog2e * tanhf(v * f[z][p & 1] / a.softcap); });
+          const float cap = a.softcap * kLog2e, squeeze = 2.f * kLog2e / a.softcap;
+          each_score([&](float v, int, int z, int p) {  // tanh x = 1 - 2 / (1 + e^2x)
+            return cap * (1.f - __fdividef(2.f, 1.f + ex2(v * f[z][p & 1] * squeeze)));
+          });
           unit_factors();
         }
         if (halves != 3u || key0 < inner_lo || key0 + kTile > inner_hi) {  // some row does not see some key
@@ -634,15 +654,14 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
                 w[x][0] = *reinterpret_cast<const uint16_t*>(from);
               }
             }
-            const __half* vs = vtab + (g * D / 256) * C::kVStride + 16 * j + 2 * c;
-            const uint32_t sa = *reinterpret_cast<const uint32_t*>(vs), sb = *reinterpret_cast<const uint32_t*>(vs + 8);
+            const uint32_t sa = vsc[j][0], sb = vsc[j][1];
 #pragma unroll
             for (int k = 0; k < kWords; ++k) {
               uint32_t even_a[4], odd_a[4], even_b[4], odd_b[4];
-              codes_to_half2((w[0][k] & 0x0f0f0f0fu) | ((w[1][k] << 4) & 0xf0f0f0f0u), even_a);
-              codes_to_half2(((w[0][k] >> 4) & 0x0f0f0f0fu) | (w[1][k] & 0xf0f0f0f0u), odd_a);
-              codes_to_half2((w[2][k] & 0x0f0f0f0fu) | ((w[3][k] << 4) & 0xf0f0f0f0u), even_b);
-              codes_to_half2(((w[2][k] >> 4) & 0x0f0f0f0fu) | (w[3][k] & 0xf0f0f0f0u), odd_b);
+              codes_to_half2(low_nibbles_of(w[0][k], w[1][k] << 4), even_a);
+              codes_to_half2(low_nibbles_of(w[0][k] >> 4, w[1][k]), odd_a);
+              codes_to_half2(low_nibbles_of(w[2][k], w[3][k] << 4), even_b);
+              codes_to_half2(low_nibbles_of(w[2][k] >> 4, w[3][k]), odd_b);
 #pragma unroll
               for (int x = 0; x < (D >= 64 ? 4 : 2); ++x) {
                 const uint32_t a0 = mul2(even_a[x], sa), a1 = mul2(odd_a[x], sa), a2 = mul2(even_b[x], sb), a3 = mul2(odd_b[x], sb);
@@ -652,32 +671,36 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
             }
           }
         };
-        if (plain && out_unit == 0) {
-          add_values();
-        } else {
-          // windows of 28 exponents, the largest first, the sums in the unit of each
-          int bias = vbias, most_byte = 254;
-          while (true) {
+        // Ordinarily one product.  Else one for each window of 28 exponents, the largest first, the sums
+        // in the unit of each.
+        const bool windows = !plain || out_unit != 0;
+        int bias = vbias, most_byte = 254;
+        while (true) {
+          bool limited = false;
+          if (windows) {
             const int got = out_unit = to_unit(acc, out_unit, bias - 112);
-            const bool limited = got != bias - 112;
+            limited = got != bias - 112;
             if (limited || bias != vbias) {
               __syncwarp();
               put_v_scales(got + 112, most_byte);
               __syncwarp();
+              get_v_scales();
             }
-            add_values();
-            if (plain || limited) break;
-            int below = 0;  // the largest byte that no window has held yet
-#pragma unroll
-            for (int x = 0; x < C::kC; ++x) {
-              const int byte = (vw >> (8 * x)) & 255;
-              if (byte <= bias && byte > 1) below = max(below, byte);
-            }
-            below = __reduce_max_sync(0xffffffffu, below);
-            if (below == 0) break;
-            most_byte = bias;
-            bias = below - 28;
           }
+          add_values();
+          if (plain || limited) break;
+          int below = 0;  // the largest byte that no window has held yet
+#pragma unroll
+          for (int x = 0; x < C::kC; ++x) {
+            const int byte = (vw >> (8 * x)) & 255;
+            if (byte <= bias && byte > 1) below = max(below, byte);
+          }
+          below = __reduce_max_sync(0xffffffffu, below);
+          if (below == 0) break;
+          most_byte = bias;
+          bias = below - 28;
+        }
+        if (!plain) {
           if (__any_sync(0xffffffffu, vnan)) {
             // a NaN block reaches the rows that see its key: this thread's dims lie in block g d/256
             for (int x = 0; x < kTile; ++x) {
@@ -783,80 +806,97 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
   }
 }
 
-// Joins the parts of one row of a segment, in their order; a segment that one block had whole is
-// done, one without keys is zero.  Warp = every eighth part, lane = D / 32 dims.
+// Joins the parts of a segment's rows, always in the same order; a segment that one block had whole
+// is done, one without keys is zero.  A block takes kRowsHere rows, so that each has 8 / kRowsHere
+// warps for its parts: one row where a segment may be cut into many parts, eight where into few.
 constexpr int kJoinWarps = 8;
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int kRowsHere>
 __global__ void __launch_bounds__(kJoinWarps * 32) fp4_attn_join_kernel(const Fp4AttnArgs a) {
-  constexpr int kX = D / 32, kRows = Cfg<D, NT>::kRows;
+  constexpr int kX = D / 32, kRows = Cfg<D, NT>::kRows, kDeep = kJoinWarps / kRowsHere;
   __shared__ float sum[kJoinWarps][D];
   __shared__ float2 ml[kJoinWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, deep = warp % kDeep;
   const int G = a.H / a.Hk;
   const int tiles_per_head = (G * a.T + kRows - 1) / kRows, row_tiles = a.Hk * tiles_per_head;
-  const int in_tile = blockIdx.x % kRows, seg = blockIdx.x / kRows, b = seg / row_tiles, y = seg % row_tiles;
+  constexpr int kPerSegment = kRows / kRowsHere;
+  const int in_tile = blockIdx.x % kPerSegment * kRowsHere + warp / kDeep;
+  const int seg = blockIdx.x / kPerSegment, b = seg / row_tiles, y = seg - b * row_tiles;
   const int i = (y % tiles_per_head) * kRows + in_tile;  // query row of the head
   const int h = y / tiles_per_head * G + i % G;
 
-  int64_t before, total;
+  int before, total;
   count_units(a, b, before, total);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (i >= G * a.T) return;
-  T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.H + h) * a.T + i / G) * D;
   if (threadIdx.x == 0 && a.lengths[b] > a.P * a.R) record_error(a.err, kErrBounds);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const Span sp = span_of(a, b);
+  T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.H + h) * a.T + i / G) * D + lane * kX;
+  const bool here = i < G * a.T;
   if (sp.tiles == 0) {
-    for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) out[d] = static_cast<T>(0.f);
+    Few<T, kX> zero;
+#pragma unroll
+    for (int d = 0; d < kX; ++d) zero.v[d] = static_cast<T>(0.f);
+    if (here && deep == 0) *reinterpret_cast<Few<T, kX>*>(out) = zero;
     return;
   }
-  const int64_t per = units_per_block(a, total * row_tiles);
-  const int64_t begin = before * row_tiles + static_cast<int64_t>(y) * units_of(sp) + kSegmentCost;  // its first tile
-  const int block0 = static_cast<int>(begin / per), block1 = static_cast<int>((begin + sp.tiles - 1) / per);
+  const int per = units_per_block(a, total * row_tiles);
+  const int begin = before * row_tiles + y * units_of(sp) + kSegmentCost;  // its first tile
+  const int block0 = begin / per, block1 = (begin + sp.tiles - 1) / per;
   if (block0 == block1) return;
 
   float top = -INFINITY, l = 0.f, o[kX] = {};
-  for (int x = block0 + warp; x <= block1; x += kJoinWarps) {
-    const int64_t slot = (static_cast<int64_t>(x) * 2 + (begin >= x * per ? 1 : 0)) * kRows + in_tile;
-    const float2 p = a.part_ml[slot];
-    const Few<float, kX> v = *reinterpret_cast<const Few<float, kX>*>(a.part_out + slot * D + lane * kX);
-    if (p.y == 0.f) continue;  // no key of this part is visible
-    const float next = fmaxf(top, p.x);
-    const float keep = l * shrink(top, next), add = p.y * shrink(p.x, next);
-    top = next;
-    l = keep + add;
-    const float old = keep / l, now = add / l;  // o is the mean so far
+  if (here) {
+#pragma unroll 4
+    for (int x = block0 + deep; x <= block1; x += kDeep) {
+      // only the first can have begun at or behind its block's first unit
+      const int64_t slot = (static_cast<int64_t>(x) * 2 + (x == block0 && begin >= x * per ? 1 : 0)) * kRows + in_tile;
+      const float2 p = a.part_ml[slot];
+      const Few<float, kX> v = *reinterpret_cast<const Few<float, kX>*>(a.part_out + slot * D + lane * kX);
+      const float next = fmaxf(top, p.x);
+      const float keep = l * shrink(top, next), add = p.y * shrink(p.x, next);  // a part without keys adds 0
+      top = next;
+      l = keep + add;
+      const float old = l == 0.f ? 0.f : keep / l, now = l == 0.f ? 0.f : add / l;  // o is the mean so far
 #pragma unroll
-    for (int d = 0; d < kX; ++d) o[d] = o[d] * old + v.v[d] * now;
+      for (int d = 0; d < kX; ++d) o[d] = o[d] * old + v.v[d] * now;
+    }
   }
+  if constexpr (kDeep > 1) {
 #pragma unroll
-  for (int d = 0; d < kX; ++d) sum[warp][lane * kX + d] = o[d];
-  if (lane == 0) ml[warp] = make_float2(top, l);
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
-    float most = -INFINITY, all = 0.f, r = 0.f;
+    for (int d = 0; d < kX; ++d) sum[warp][lane * kX + d] = o[d];
+    if (lane == 0) ml[warp] = make_float2(top, l);
+    __syncthreads();
+    if (deep != 0) return;
+    for (int w = warp + 1; w < warp + kDeep; ++w) {
+      const float2 p = ml[w];
+      const float next = fmaxf(top, p.x);
+      const float keep = l * shrink(top, next), add = p.y * shrink(p.x, next);
+      top = next;
+      l = keep + add;
+      const float old = l == 0.f ? 0.f : keep / l, now = l == 0.f ? 0.f : add / l;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) most = fmaxf(most, ml[w].x);
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w)
-      if (ml[w].y != 0.f) all += ml[w].y * shrink(ml[w].x, most);
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w)
-      if (ml[w].y != 0.f) r += sum[w][d] * (ml[w].y * shrink(ml[w].x, most) / all);
-    if (a.sink != nullptr) r *= share_beside(a.sink[h], most, all);
-    out[d] = static_cast<T>(r);
+      for (int d = 0; d < kX; ++d) o[d] = o[d] * old + sum[w][lane * kX + d] * now;
+    }
   }
+  if (!here) return;
+  const float keep = a.sink != nullptr ? share_beside(a.sink[h], top, l) : 1.f;
+  Few<T, kX> r;
+#pragma unroll
+  for (int d = 0; d < kX; ++d) r.v[d] = static_cast<T>(o[d] * keep);
+  *reinterpret_cast<Few<T, kX>*>(out) = r;
 }
 
 template <typename T, int D, int NT>
-void launch(Fp4AttnArgs& a, cudaStream_t stream) {
+void launch(const Fp4AttnArgs& a, cudaStream_t stream) {
   using C = Cfg<D, NT>;
   const int64_t segments = fp4_attn_segments(a);
   cudaFuncSetAttribute(fp4_attn_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   fp4_attn_rows_kernel<T, D, NT><<<a.blocks, kWarps * 32, C::kSmem, stream>>>(a);
   // the join may start while the last blocks run: it waits where it reads their parts
   cudaLaunchConfig_t join{};
-  join.gridDim = dim3(static_cast<unsigned>(segments * C::kRows));
+  // parts per segment: 16 or more take a block for each row (batch of 64: 1024 blocks 12 us, 128 blocks 6 us)
+  const bool deep = a.blocks >= 16 * segments;
+  join.gridDim = dim3(static_cast<unsigned>(segments * C::kRows / (deep ? 1 : 8)));
   join.blockDim = dim3(kJoinWarps * 32);
   join.stream = stream;
   cudaLaunchAttribute early{};
@@ -864,11 +904,12 @@ void launch(Fp4AttnArgs& a, cudaStream_t stream) {
   early.val.programmaticStreamSerializationAllowed = 1;
   join.attrs = &early;
   join.numAttrs = 1;
-  cudaLaunchKernelEx(&join, fp4_attn_join_kernel<T, D, NT>, static_cast<const Fp4AttnArgs&>(a));
+  if (deep) cudaLaunchKernelEx(&join, fp4_attn_join_kernel<T, D, NT, 1>, a);
+  else cudaLaunchKernelEx(&join, fp4_attn_join_kernel<T, D, NT, 8>, a);
 }
 
 template <typename T>
-void by_shape(Fp4AttnArgs& a, int d, cudaStream_t stream) {
+void by_shape(const Fp4AttnArgs& a, int d, cudaStream_t stream) {
   const bool few = fp4_attn_rows_per_segment(a) == 8;
   if (d == 32) few ? launch<T, 32, 1>(a, stream) : launch<T, 32, 2>(a, stream);
   else if (d == 64) few ? launch<T, 64, 1>(a, stream) : launch<T, 64, 2>(a, stream);
@@ -884,14 +925,17 @@ int64_t fp4_attn_segments(const Fp4AttnArgs& a) {
   return static_cast<int64_t>(a.B) * a.Hk * ((static_cast<int64_t>(a.H / a.Hk) * a.T + rows - 1) / rows);
 }
 
-int fp4_attn_blocks(const Fp4AttnArgs& a, int d) {
+int64_t fp4_attn_units(const Fp4AttnArgs& a) {
   const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.P) * a.R, a.window > 0 ? static_cast<int64_t>(a.window) + a.T + 31 : INT32_MAX);
-  const int64_t units = fp4_attn_segments(a) * ((keys + kTile - 1) / kTile + kSegmentCost);
-  const int64_t wave = 148 * (d == 128 && fp4_attn_rows_per_segment(a) == 16 ? 3 : 4);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wave, (units + kWarps - 1) / kWarps)));
+  return fp4_attn_segments(a) * ((keys + kTile - 1) / kTile + kSegmentCost);
 }
 
-void fp4_attn_rows(Fp4AttnArgs& a, int d, bool half, cudaStream_t stream) {
+int fp4_attn_blocks(const Fp4AttnArgs& a, int d) {
+  const int64_t wave = 148 * (d == 128 && fp4_attn_rows_per_segment(a) == 16 ? 2 : 4);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wave, (fp4_attn_units(a) + kWarps - 1) / kWarps)));
+}
+
+void fp4_attn_rows(const Fp4AttnArgs& a, int d, bool half, cudaStream_t stream) {
   if (half) by_shape<__half>(a, d, stream);
   else by_shape<__nv_bfloat16>(a, d, stream);
 }

@@ -307,7 +307,7 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   a.softcap = static_cast<float>(softcap);
   a.err = err.data_ptr<int>();
   TORCH_CHECK(B <= 65535 && H * T <= (1 << 26), "fp4_kv_attention: at most 65535 sequences and 2^26 query rows in each");
-  TORCH_CHECK(fp4_attn_segments(a) * 16 < INT32_MAX, "fp4_kv_attention: too many query rows");
+  TORCH_CHECK(fp4_attn_units(a) < INT32_MAX, "fp4_kv_attention: more than 2^31 tiles of work in one call");
   a.blocks = fp4_attn_blocks(a, static_cast<int>(d));
   const int64_t part_rows = static_cast<int64_t>(a.blocks) * 2 * fp4_attn_rows_per_segment(a);
   torch::Tensor parts = torch::empty({part_rows * (d + 2)}, q.options().dtype(at::kFloat));

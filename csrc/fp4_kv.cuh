@@ -31,13 +31,14 @@ struct Fp4AttnArgs {
   int* err;
 };
 
-// Query rows (heads of a K / V head times tokens) of one unit of work, the number of those units
-// (sequence, K / V head, rows), and the blocks of one wave for head_dim d.
+// Query rows (heads of a K / V head times tokens) of one segment of work, the number of segments
+// (sequence, K / V head, rows), a bound on the units of work in all, and the blocks of one wave.
 int fp4_attn_rows_per_segment(const Fp4AttnArgs& a);
 int64_t fp4_attn_segments(const Fp4AttnArgs& a);
+int64_t fp4_attn_units(const Fp4AttnArgs& a);
 int fp4_attn_blocks(const Fp4AttnArgs& a, int d);
 
 // Launch for head_dim d (32, 64, 128) and q in fp16 or bf16.
-void fp4_attn_rows(Fp4AttnArgs& a, int d, bool half, cudaStream_t stream);
+void fp4_attn_rows(const Fp4AttnArgs& a, int d, bool half, cudaStream_t stream);
 
 }  // namespace sv4
