@@ -43,7 +43,8 @@ void grouped_gemm_fp8(int64_t mode, torch::Tensor a, torch::Tensor sfa, torch::T
                       int64_t n_probs, int64_t b_rows, double gmax, double lo, double hi, torch::Tensor err);
 // fp4_kv.cu
 void fp4_kv_write(torch::Tensor k, torch::Tensor v, torch::Tensor pages, torch::Tensor slots, torch::Tensor err);
-void fp4_kv_read(torch::Tensor pages, torch::Tensor slots, torch::Tensor k, torch::Tensor v, torch::Tensor err);
+std::tuple<torch::Tensor, torch::Tensor> fp4_kv_read(torch::Tensor pages, torch::Tensor slots, int64_t d,
+                                                     at::ScalarType dtype, torch::Tensor err);
 torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tensor table, torch::Tensor lengths,
                                int64_t window, c10::optional<torch::Tensor> sink, double softcap, double scale,
                                torch::Tensor err);

@@ -1,6 +1,7 @@
 // A paged K / V cache held in 4 bits (MXFP4): rows quantised into pages, rows read back, and
 // attention that reads the pages as they are (fp4_attn.cu).  The page format: fp4_kv.cuh.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -10,7 +11,6 @@
 namespace sv4 {
 namespace {
 
-constexpr int kBlock = 32;  // values that share a scale
 
 template <typename T>
 __device__ __forceinline__ float as_float(T v);
@@ -40,15 +40,50 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
 }
 
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-  const uint32_t two = (code >> 1) & 3u, m = code & 1u;
-  const float mag = two == 0 ? 0.5f * m : __uint_as_float(((two + 126u) << 23) | (m << 22));
-  return (code & 8u) ? -mag : mag;
+// Eight values (in units of the scale) as E2M1 codes, the first in the lowest four bits.  cvt rounds
+// ties to the even code, the format to the smaller one: they differ at 0.75, 1.75 and 3.5.  Values
+// of 16-bit types have eleven bits or fewer, so a factor of 1 - 2^-20 (in `inv`) puts ties, and
+// nothing else, below themselves; fp32 values are compared.  A negative zero becomes zero.
+template <typename T>
+__device__ __forceinline__ uint32_t e2m1_codes(const float (&f)[8], float inv) {
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = f[j] * (sizeof(T) == 2 ? inv * (1.f - 0x1p-20f) : inv);
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w) : "f"(a[0]), "f"(a[1]), "f"(a[2]), "f"(a[3]), "f"(a[4]), "f"(a[5]), "f"(a[6]), "f"(a[7]));
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float m = fabsf(a[j]);
+      if (m == 0.75f || m == 1.75f || m == 3.5f) w -= 1u << (4 * j);
+    }
+  }
+  const uint32_t some = ((w & 0x77777777u) + 0x77777777u) & 0x88888888u;  // the sign bit where the magnitude is not 0
+  return w & (some | 0x77777777u);
 }
 
-// Nearest E2M1 magnitude of a >= 0 (in units of the scale), a tie going to the smaller one.
-__device__ __forceinline__ uint32_t e2m1_code(float a) {
-  return (a > 0.25f) + (a > 0.75f) + (a > 1.25f) + (a > 1.75f) + (a > 2.5f) + (a > 3.5f) + (a > 5.0f);
+// Eight codes -> values.
+__device__ __forceinline__ void e2m1_values(uint32_t w, float (&f)[8]) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+    f[2 * j] = v.x;
+    f[2 * j + 1] = v.y;
+  }
 }
 
 struct RowsArgs {
@@ -64,79 +99,93 @@ struct RowsArgs {
   int* err;
 };
 
-// Thread = eight values of one row; four neighbouring threads share a scale.
+// Where a slot's row lies: its page's slab of `head`, and the row in it; null: skipped.
+__device__ __forceinline__ uint8_t* slab_of(const RowsArgs& a, int64_t slot, int head, int& r) {
+  r = 0;
+  if (slot == -1 || !index_ok(slot, 0, a.n_slots, a.err)) return nullptr;
+  int64_t page;
+  if (a.n_slots <= UINT32_MAX) page = static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.R);
+  else page = slot / a.R;
+  r = static_cast<int>(slot - page * a.R);
+  return a.pages + page * a.page_stride + static_cast<int64_t>(head) * a.slab;
+}
+
+// Both kernels move bytes (16.5 to 32.5 bits a value) and are bound by them: one thread handles
+// eight values of a row, so that accesses are 16 (rows) and 4 bytes (codes) wide, of kUnroll rows,
+// whose loads are all in flight before the first is used.  Block y is a head's K or V.
+constexpr int kRowThreads = 256, kUnroll = 4;
+
+// Four neighbouring threads share a scale: the largest magnitude over them.
 template <typename T, int D>
-__global__ void fp4_kv_write_kernel(const RowsArgs a) {
-  constexpr int kPer = D / 8;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int part = static_cast<int>(i % kPer);
-  const int64_t unit = i / kPer;
-  const int kv = static_cast<int>(unit & 1);
-  const int head = static_cast<int>((unit >> 1) % a.heads);
-  const int64_t row = (unit >> 1) / a.heads;
-  const int64_t slot = row < a.rows ? a.slots[row] : -1;
-  // rows that are skipped keep their lanes for the shuffles
-  const bool live = slot != -1 && row < a.rows && index_ok(slot, 0, a.n_slots, a.err);
-  Eight<T> x;
-  float f[8];
-  float amax = 0.f;
-  if (live) {
-    x = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(a.src[kv]) + row * a.row_stride[kv] +
-                                           head * a.head_stride[kv] + part * 8);
+__global__ void __launch_bounds__(kRowThreads) fp4_kv_write_kernel(const RowsArgs a) {
+  constexpr int kPer = D / 8, kRows = kRowThreads / kPer;
+  const int part = threadIdx.x % kPer, kv = blockIdx.y & 1, head = blockIdx.y >> 1;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kRows * kUnroll) + threadIdx.x / kPer;
+  const T* src = static_cast<const T*>(a.src[kv]) + head * a.head_stride[kv] + part * 8;
+  int64_t slot[kUnroll];
+  Eight<T> x[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t row = row0 + u * kRows;
+    slot[u] = row < a.rows ? a.slots[row] : -1;
+    if (row < a.rows) x[u] = *reinterpret_cast<const Eight<T>*>(src + row * a.row_stride[kv]);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    int r;
+    uint8_t* slab = slab_of(a, slot[u], head, r);
+    float f[8], amax = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      f[j] = as_float<T>(x.v[j]);
-      const float m = fabsf(f[j]);
-      amax = m <= 3.402823466e38f ? fmaxf(amax, m) : INFINITY;  // a NaN must not be dropped by fmaxf
-      if (isinf(amax)) break;
+      f[j] = slab != nullptr ? as_float<T>(x[u].v[j]) : 0.f;
+      amax = fmaxf(amax, fabsf(f[j]) <= 3.402823466e38f ? fabsf(f[j]) : INFINITY);  // fmaxf would drop a NaN
     }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    if (slab == nullptr) continue;
+    const uint32_t bits = __float_as_uint(amax);
+    // amax = 1.m * 2^x: the exponent is x - 2 while 1.m <= 1.5
+    const int e = max(-126, static_cast<int>(bits >> 23) - 129 + ((bits & 0x7fffffu) > 0x400000u ? 1 : 0));
+    const bool bad = isinf(amax);
+    const uint32_t word = bad ? 0u : e2m1_codes<T>(f, __uint_as_float(static_cast<uint32_t>(127 - e) << 23));
+    *reinterpret_cast<uint32_t*>(slab + (kv * a.R + r) * (D / 2) + part * 4) = word;
+    if ((part & 3) == 0) slab[a.R * D + (kv * a.R + r) * (D / 32) + part / 4] = static_cast<uint8_t>(bad ? 255 : e + 127);
   }
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  if (!live) return;
-  const uint32_t bits = __float_as_uint(amax);
-  // amax = 1.m * 2^x: the exponent is x - 2 while 1.m <= 1.5
-  const int e = max(-126, static_cast<int>(bits >> 23) - 129 + ((bits & 0x7fffffu) > 0x400000u ? 1 : 0));
-  const bool bad = isinf(amax);
-  const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  uint32_t word = 0;
-  if (!bad) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t c = e2m1_code(fabsf(f[j]) * inv);
-      word |= (c | (f[j] < 0.f && c != 0 ? 8u : 0u)) << (4 * j);
-    }
-  }
-  const int64_t page = slot / a.R;
-  const int r = static_cast<int>(slot % a.R);
-  uint8_t* slab = a.pages + page * a.page_stride + static_cast<int64_t>(head) * a.slab;
-  *reinterpret_cast<uint32_t*>(slab + (kv * a.R + r) * (D / 2) + part * 4) = word;
-  if ((part & 3) == 0) slab[a.R * D + (kv * a.R + r) * (D / 32) + part / 4] = static_cast<uint8_t>(bad ? 255 : e + 127);
 }
 
 template <typename T, int D>
-__global__ void fp4_kv_read_kernel(const RowsArgs a) {
-  constexpr int kPer = D / 8;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int part = static_cast<int>(i % kPer);
-  const int64_t unit = i / kPer;
-  const int kv = static_cast<int>(unit & 1);
-  const int head = static_cast<int>((unit >> 1) % a.heads);
-  const int64_t row = (unit >> 1) / a.heads;
-  if (row >= a.rows) return;
-  const int64_t slot = a.slots[row];
-  Eight<T> y;
-  uint32_t word = 0;
-  float s = 0.f;
-  if (slot != -1 && index_ok(slot, 0, a.n_slots, a.err)) {
-    const int r = static_cast<int>(slot % a.R);
-    const uint8_t* slab = a.pages + slot / a.R * a.page_stride + static_cast<int64_t>(head) * a.slab;
-    word = *reinterpret_cast<const uint32_t*>(slab + (kv * a.R + r) * (D / 2) + part * 4);
-    s = scale_of(slab[a.R * D + (kv * a.R + r) * (D / 32) + part / 4]);
+__global__ void __launch_bounds__(kRowThreads) fp4_kv_read_kernel(const RowsArgs a) {
+  constexpr int kPer = D / 8, kRows = kRowThreads / kPer;
+  const int part = threadIdx.x % kPer, kv = blockIdx.y & 1, head = blockIdx.y >> 1;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kRows * kUnroll) + threadIdx.x / kPer;
+  int64_t slot[kUnroll];
+  uint32_t word[kUnroll];
+  uint8_t byte[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) slot[u] = row0 + u * kRows < a.rows ? a.slots[row0 + u * kRows] : -1;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    int r;
+    const uint8_t* slab = slab_of(a, slot[u], head, r);
+    word[u] = 0;
+    byte[u] = 127;
+    if (slab != nullptr) {
+      word[u] = *reinterpret_cast<const uint32_t*>(slab + (kv * a.R + r) * (D / 2) + part * 4);
+      byte[u] = slab[a.R * D + (kv * a.R + r) * (D / 32) + part / 4];
+    }
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y.v[j] = from_float<T>(e2m1_value((word >> (4 * j)) & 15u) * s);
-  *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.dst[kv]) + ((row * a.heads + head) * D + part * 8)) = y;
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t row = row0 + u * kRows;
+    if (row >= a.rows) continue;
+    float f[8];
+    e2m1_values(word[u], f);
+    const float s = scale_of(byte[u]);
+    Eight<T> y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y.v[j] = from_float<T>(f[j] * s);
+    *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.dst[kv]) + ((row * a.heads + head) * D + part * 8)) = y;
+  }
 }
 
 // Numbers in messages go through std::to_string: the stream operators of the toolchain's
@@ -192,9 +241,20 @@ RowsArgs rows_args(const torch::Tensor& pages, const torch::Tensor& slots, int64
   a.slots = slots.data_ptr<int64_t>();
   a.rows = slots.size(0);
   a.n_slots = pages.size(0) * a.R;
+  TORCH_CHECK(pages.size(1) <= 32767, who, ": at most 32767 K/V heads");
   a.heads = static_cast<int>(pages.size(1));
   a.slab = static_cast<int>(pages.size(2));
   return a;
+}
+
+// A tensor on like's device, without the dispatcher's cost (the calls are short).
+torch::Tensor uninitialised(at::IntArrayRef sizes, at::ScalarType dtype, const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
+}
+
+dim3 rows_grid(const RowsArgs& a, int64_t d) {
+  const int64_t per = kRowThreads / (d / 8) * kUnroll;
+  return dim3(static_cast<unsigned>((a.rows + per - 1) / per), static_cast<unsigned>(2 * a.heads));
 }
 
 }  // namespace
@@ -210,7 +270,7 @@ void fp4_kv_write(torch::Tensor k, torch::Tensor v, torch::Tensor pages, torch::
   RowsArgs a = rows_args(pages, slots, d, "fp4_kv_write");
   TORCH_CHECK(k.size(1) == a.heads && k.size(0) == a.rows, "fp4_kv_write: ", num(k.size(0)), " rows of ",
               num(k.size(1)), " heads for ", num(a.rows), " slots and pages of ", num(a.heads), " heads");
-  if (a.rows == 0) return;
+  if (k.numel() == 0) return;
   c10::cuda::CUDAGuard guard(k.device());
   k = rows_aligned(k);
   v = rows_aligned(v);
@@ -221,41 +281,37 @@ void fp4_kv_write(torch::Tensor k, torch::Tensor v, torch::Tensor pages, torch::
   a.head_stride[0] = k.stride(1);
   a.head_stride[1] = v.stride(1);
   a.err = err.data_ptr<int>();
-  const int64_t threads = a.rows * a.heads * 2 * (d / 8);
-  const unsigned grid = static_cast<unsigned>((threads + 255) / 256);
+  const dim3 grid = rows_grid(a, d);
   auto stream = at::cuda::getCurrentCUDAStream();
   by_dim(d, [&](auto dim) {
     by_type(k.scalar_type(), [&](auto t) {
-      fp4_kv_write_kernel<decltype(t), decltype(dim)::value><<<grid, 256, 0, stream>>>(a);
+      fp4_kv_write_kernel<decltype(t), decltype(dim)::value><<<grid, kRowThreads, 0, stream>>>(a);
     });
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// The rows at `slots` as k, v (N, kv_heads, d); a slot of -1 gives zeros.
-void fp4_kv_read(torch::Tensor pages, torch::Tensor slots, torch::Tensor k, torch::Tensor v, torch::Tensor err) {
-  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && k.scalar_type() == v.scalar_type() && k.is_contiguous() &&
-                  v.is_contiguous() && k.device() == pages.device() && v.device() == pages.device(),
-              "fp4_kv_read: outputs must be contiguous (rows, kv_heads, head_dim) of one type on the pages' device");
-  TORCH_CHECK(k.scalar_type() == at::kFloat || k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16,
-              "fp4_kv_read: rows must be bf16, fp16 or fp32");
-  const int64_t d = k.size(2);
+// The rows at `slots` as k, v (N, kv_heads, d) of type `dtype`; a slot of -1 gives zeros.
+std::tuple<torch::Tensor, torch::Tensor> fp4_kv_read(torch::Tensor pages, torch::Tensor slots, int64_t d,
+                                                     at::ScalarType dtype, torch::Tensor err) {
+  TORCH_CHECK(dtype == at::kFloat || dtype == at::kHalf || dtype == at::kBFloat16,
+              "fp4_kv_read: rows are read in bf16, fp16 or fp32");
   RowsArgs a = rows_args(pages, slots, d, "fp4_kv_read");
-  TORCH_CHECK(k.size(1) == a.heads && k.size(0) == a.rows, "fp4_kv_read: outputs do not match slots and pages");
-  if (a.rows == 0) return;
-  c10::cuda::CUDAGuard guard(k.device());
+  c10::cuda::CUDAGuard guard(pages.device());
+  auto k = uninitialised({a.rows, a.heads, d}, dtype, pages), v = uninitialised({a.rows, a.heads, d}, dtype, pages);
+  if (k.numel() == 0) return {k, v};
   a.dst[0] = k.data_ptr();
   a.dst[1] = v.data_ptr();
   a.err = err.data_ptr<int>();
-  const int64_t threads = a.rows * a.heads * 2 * (d / 8);
-  const unsigned grid = static_cast<unsigned>((threads + 255) / 256);
+  const dim3 grid = rows_grid(a, d);
   auto stream = at::cuda::getCurrentCUDAStream();
   by_dim(d, [&](auto dim) {
     by_type(k.scalar_type(), [&](auto t) {
-      fp4_kv_read_kernel<decltype(t), decltype(dim)::value><<<grid, 256, 0, stream>>>(a);
+      fp4_kv_read_kernel<decltype(t), decltype(dim)::value><<<grid, kRowThreads, 0, stream>>>(a);
     });
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {k, v};
 }
 
 // q (B, H, T, d) bf16 / fp16; table (B, P) int32; lengths (B) int32, the T tokens included.
@@ -282,7 +338,7 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
     TORCH_CHECK(sink->scalar_type() == at::kFloat && sink->numel() == H && sink->is_contiguous() &&
                     sink->device() == q.device(), "fp4_kv_attention: sink must be ", num(H), " contiguous fp32 values");
   c10::cuda::CUDAGuard guard(q.device());
-  torch::Tensor out = torch::empty({B, H, T, d}, q.options());
+  torch::Tensor out = uninitialised({B, H, T, d}, q.scalar_type(), q);
   if (out.numel() == 0) return out;
   q = rows_aligned(q);
   a.q = q.data_ptr();
@@ -310,7 +366,7 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   TORCH_CHECK(fp4_attn_units(a) < INT32_MAX, "fp4_kv_attention: more than 2^31 tiles of work in one call");
   a.blocks = fp4_attn_blocks(a, static_cast<int>(d));
   const int64_t part_rows = static_cast<int64_t>(a.blocks) * 2 * fp4_attn_rows_per_segment(a);
-  torch::Tensor parts = torch::empty({part_rows * (d + 2)}, q.options().dtype(at::kFloat));
+  torch::Tensor parts = uninitialised({part_rows * (d + 2)}, at::kFloat, q);
   a.part_ml = reinterpret_cast<float2*>(parts.data_ptr<float>());
   a.part_out = parts.data_ptr<float>() + 2 * part_rows;
   fp4_attn_rows(a, static_cast<int>(d), q.scalar_type() == at::kHalf, at::cuda::getCurrentCUDAStream());

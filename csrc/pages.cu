@@ -5,6 +5,7 @@
 // State: table (S, P) int32 page ids, -1 behind a row's last page; lengths (S) rows;
 // refcount (n_pages) rows of the table that hold a page, 0 = free.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -42,6 +43,27 @@ __device__ __forceinline__ int block_scan(int v, int* total) {
   return x - v + (warp > 0 ? sums[warp - 1] : 0);
 }
 
+// The second kernel of a pair may be set up while the first runs, and waits for its results.
+__device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+constexpr int kCopyThreads = 256, kPiece = 16384;  // bytes: four 16-byte loads in flight per thread
+
+// Up to kPiece bytes (a multiple of 16) by the whole block.
+__device__ __forceinline__ void copy_piece(uint8_t* to, const uint8_t* from, int64_t bytes) {
+  const uint4* src = reinterpret_cast<const uint4*>(from);
+  uint4* dst = reinterpret_cast<uint4*>(to);
+  constexpr int kEach = kPiece / 16 / kCopyThreads;
+  const int n = static_cast<int>(bytes / 16);
+  uint4 v[kEach];
+#pragma unroll
+  for (int x = 0; x < kEach; ++x)
+    if (static_cast<int>(threadIdx.x) + x * kCopyThreads < n) v[x] = src[threadIdx.x + x * kCopyThreads];
+#pragma unroll
+  for (int x = 0; x < kEach; ++x)
+    if (static_cast<int>(threadIdx.x) + x * kCopyThreads < n) dst[threadIdx.x + x * kCopyThreads] = v[x];
+}
+
 struct ForkArgs {
   uint8_t* pool;
   int64_t page_bytes;
@@ -74,6 +96,7 @@ __device__ __forceinline__ bool fork_rows(const ForkArgs& a, int i, int* err, in
 // Block 0 gives every fork that copies a tail the next free page in ascending order; the other
 // blocks copy the state that the forks then change.
 __global__ void __launch_bounds__(kPlan) fork_plan_kernel(const ForkArgs a) {
+  release_next();
   if (blockIdx.x > 0) {
     const int64_t step = static_cast<int64_t>(gridDim.x - 1) * kPlan;
     const int64_t first = static_cast<int64_t>(blockIdx.x - 1) * kPlan + threadIdx.x;
@@ -112,10 +135,11 @@ __global__ void __launch_bounds__(kPlan) fork_plan_kernel(const ForkArgs a) {
   if (threadIdx.x == 0) a.fresh[a.F] = fits;
 }
 
-// Block (i, y): fork i.  Every block copies its part of the tail page; block y = 0 also rewrites
+// Block (i, y): fork i.  Every block copies pieces of the tail page; block y = 0 also rewrites
 // the child's row and counts the pages that it leaves and takes (sums of whole numbers: their
 // order does not matter).
-__global__ void __launch_bounds__(256) fork_apply_kernel(const ForkArgs a) {
+__global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(const ForkArgs a) {
+  wait_previous();
   if (a.fresh[a.F] == 0) return;  // too few free pages: nothing changes
   const int i = blockIdx.x;
   int parent, child, len;
@@ -139,12 +163,9 @@ __global__ void __launch_bounds__(256) fork_apply_kernel(const ForkArgs a) {
   if (fresh < 0) return;
   const int source = from[tail];
   if (!index_ok(source, 0, a.n_pages, a.err)) return;
-  const uint4* src = reinterpret_cast<const uint4*>(a.pool + source * a.page_bytes);
-  uint4* dst = reinterpret_cast<uint4*>(a.pool + fresh * a.page_bytes);
-  const int64_t n = a.page_bytes / 16;
-  for (int64_t x = static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x; x < n;
-       x += static_cast<int64_t>(gridDim.y) * blockDim.x)
-    dst[x] = src[x];
+  for (int64_t at = static_cast<int64_t>(blockIdx.y) * kPiece; at < a.page_bytes; at += static_cast<int64_t>(gridDim.y) * kPiece)
+    copy_piece(a.pool + fresh * a.page_bytes + at, a.pool + source * a.page_bytes + at,
+               min(static_cast<int64_t>(kPiece), a.page_bytes - at));
 }
 
 struct CompactArgs {
@@ -156,40 +177,61 @@ struct CompactArgs {
   int* new_refcount;
   int* live;   // scalar: pages in use
   int* where;  // (n_pages): where a page's contents go; -1: free
-  int* moves;  // (2, n_pages): k-th hole below the live count, k-th live page from it on
+  int* moves;  // count, then (target, source) pairs
   int64_t entries;
   int n_pages;
   int* err;
 };
 
+// One block: a thread classifies four neighbouring pages, two counts share a scan.  The k-th hole
+// below the live count takes the k-th live page from it on.
 __global__ void __launch_bounds__(kPlan) compact_plan_kernel(const CompactArgs a) {
-  int live = 0;
-  for (int p0 = 0; p0 < a.n_pages; p0 += kPlan) {
-    const int p = p0 + threadIdx.x;
-    live += __syncthreads_count(p < a.n_pages && a.refcount[p] > 0);
-  }
+  __shared__ int live_s;
+  release_next();
+  if (threadIdx.x == 0) live_s = 0;
+  __syncthreads();
+  int mine = 0;
+  for (int p = threadIdx.x; p < a.n_pages; p += kPlan) mine += a.refcount[p] > 0;
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if ((threadIdx.x & 31) == 0) atomicAdd(&live_s, mine);
+  __syncthreads();
+  const int live = live_s;
   if (threadIdx.x == 0) *a.live = live;
-  int* hole = a.moves;
-  int* late = a.moves + a.n_pages;
+  int* target = a.moves + 1;
+  int* source = a.moves + 1 + a.n_pages;
   int holes = 0, lates = 0;
-  for (int p0 = 0; p0 < a.n_pages; p0 += kPlan) {
-    const int p = p0 + threadIdx.x;
-    const bool in = p < a.n_pages, used = in && a.refcount[p] > 0;
+  for (int p0 = 0; p0 < a.n_pages; p0 += 4 * kPlan) {
+    const int p = p0 + 4 * threadIdx.x;
+    uint32_t counts = 0;  // holes in the low half, late pages in the high half: at most 4096 each
+    bool hole[4], late[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const bool in = p + x < a.n_pages, used = in && a.refcount[p + x] > 0;
+      hole[x] = in && !used && p + x < live;
+      late[x] = used && p + x >= live;
+      if (in) a.where[p + x] = used && !late[x] ? p + x : -1;
+      counts += (hole[x] ? 1u : 0u) + (late[x] ? 0x10000u : 0u);
+    }
     int total;
-    const int h = block_scan(in && !used && p < live, &total) + holes;
-    holes += total;
-    const int t = block_scan(used && p >= live, &total) + lates;
-    lates += total;
-    if (in && !used && p < live) hole[h] = p;
-    if (used && p >= live) late[t] = p;
-    if (in) a.where[p] = used && p < live ? p : -1;
+    const uint32_t before = block_scan(static_cast<int>(counts), &total);
+    int h = holes + (before & 0xffffu), t = lates + (before >> 16);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (hole[x]) target[h++] = p + x;
+      if (late[x]) source[t++] = p + x;
+    }
+    holes += total & 0xffff;
+    lates += static_cast<uint32_t>(total) >> 16;
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < lates; k += kPlan) a.where[late[k]] = hole[k];
+  for (int k = threadIdx.x; k < lates; k += kPlan) a.where[source[k]] = target[k];
+  if (threadIdx.x == 0) a.moves[0] = lates;
 }
 
 // Sources are at or behind the live count and targets before it, so the copies are independent.
-__global__ void __launch_bounds__(256) compact_apply_kernel(const CompactArgs a) {
+// Bound by the pool's bytes: blocks take 16 KB pieces of the moved pages in turn.
+__global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const CompactArgs a) {
+  wait_previous();
   const int live = *a.live;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -202,14 +244,31 @@ __global__ void __launch_bounds__(256) compact_apply_kernel(const CompactArgs a)
     if (p >= live) a.new_refcount[p] = 0;
     if (to >= 0) a.new_refcount[to] = a.refcount[p];
   }
-  const int64_t n = a.page_bytes / 16;
-  for (int p = live + blockIdx.x; p < a.n_pages; p += gridDim.x) {
-    const int to = a.where[p];
-    if (to < 0) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(a.pool + p * a.page_bytes);
-    uint4* dst = reinterpret_cast<uint4*>(a.pool + to * a.page_bytes);
-    for (int64_t x = threadIdx.x; x < n; x += blockDim.x) dst[x] = src[x];
+  const int64_t pieces = (a.page_bytes + kPiece - 1) / kPiece, n = a.moves[0] * pieces;
+  for (int64_t x = blockIdx.x; x < n; x += gridDim.x) {
+    const int64_t k = x / pieces, at = (x - k * pieces) * kPiece;
+    copy_piece(a.pool + a.moves[1 + k] * a.page_bytes + at, a.pool + a.moves[1 + a.n_pages + k] * a.page_bytes + at,
+               min(static_cast<int64_t>(kPiece), a.page_bytes - at));
   }
+}
+
+// An int32 tensor like `like`, without the dispatcher's cost (the calls are short).
+torch::Tensor ints(at::IntArrayRef sizes, const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, at::kInt, like.device(), std::nullopt);
+}
+
+template <typename A>
+void launch_after(void (*kernel)(A), dim3 grid, const A& args, cudaStream_t stream) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(kCopyThreads);
+  config.stream = stream;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args));
 }
 
 // The pool as pages of bytes; returns the bytes of a page.
@@ -245,8 +304,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> fork_pages(torch::Tensor
   TORCH_CHECK(page_rows > 0 && table.size(1) * page_rows <= INT32_MAX, "fork_pages: page_rows must be positive");
   c10::cuda::CUDAGuard guard(pool.device());
   if (F == 0) return {table.clone(), lengths.clone(), refcount.clone()};
-  auto new_table = torch::empty_like(table), new_lengths = torch::empty_like(lengths), new_refs = torch::empty_like(refcount);
-  auto fresh = torch::empty({2 * F + 1}, table.options());
+  auto new_table = ints(table.sizes(), table), new_lengths = ints(lengths.sizes(), table), new_refs = ints(refcount.sizes(), table);
+  auto fresh = ints({2 * F + 1}, table);
   a.pool = static_cast<uint8_t*>(pool.data_ptr());
   a.table = table.data_ptr<int>();
   a.lengths = lengths.data_ptr<int>();
@@ -267,9 +326,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> fork_pages(torch::Tensor
   auto stream = at::cuda::getCurrentCUDAStream();
   fork_plan_kernel<<<1 + static_cast<unsigned>(std::min<int64_t>(147, (copied + kPlan - 1) / kPlan)), kPlan, 0, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(64, a.page_bytes / 16384));
-  fork_apply_kernel<<<dim3(static_cast<unsigned>(F), static_cast<unsigned>(parts)), 256, 0, stream>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(64, (a.page_bytes + kPiece - 1) / kPiece));
+  launch_after(fork_apply_kernel, dim3(static_cast<unsigned>(F), static_cast<unsigned>(pieces)), a, stream);
   return {new_table, new_lengths, new_refs};
 }
 
@@ -278,10 +336,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> compact_pages(torch::Ten
   CompactArgs a{};
   a.page_bytes = check_pool(pool, table, refcount, "compact_pages");
   c10::cuda::CUDAGuard guard(pool.device());
-  auto new_table = torch::empty_like(table), new_refs = torch::empty_like(refcount);
-  auto live = torch::empty({}, table.options());
+  auto new_table = ints(table.sizes(), table), new_refs = ints(refcount.sizes(), table), live = ints({}, table);
   if (pool.size(0) == 0) return {table.clone(), new_refs, live.zero_()};
-  auto work = torch::empty({3 * pool.size(0)}, table.options());
+  auto work = ints({3 * pool.size(0) + 1}, table);
   a.pool = static_cast<uint8_t*>(pool.data_ptr());
   a.table = table.data_ptr<int>();
   a.refcount = refcount.data_ptr<int>();
@@ -296,8 +353,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> compact_pages(torch::Ten
   auto stream = at::cuda::getCurrentCUDAStream();
   compact_plan_kernel<<<1, kPlan, 0, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  compact_apply_kernel<<<148 * 4, 256, 0, stream>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_after(compact_apply_kernel, dim3(148 * 8), a, stream);
   return {new_table, new_refs, live};
 }
 

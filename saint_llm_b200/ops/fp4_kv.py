@@ -27,6 +27,7 @@ import torch
 from torch import Tensor
 
 from saint_llm_b200.ops import backend
+from saint_llm_b200.ops.gemm import error_word
 from saint_llm_b200.ops.quant import FP4_E2M1_LEVELS
 
 BLOCK = 32
@@ -95,8 +96,6 @@ def fp4_kv_write(k: Tensor, v: Tensor, pages: Tensor, slots: Tensor) -> None:
     ``pages`` at ``slots`` (N,) int64 = page * page_rows + row, in place.  -1 skips a row; the
     other slots must differ from one another."""
     if backend.native_for(pages):
-        from saint_llm_b200.ops.gemm import error_word
-
         backend.ext().fp4_kv_write(k, v, pages, slots, error_word(pages.device))
         return
     if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _ROW_TYPES:
@@ -116,12 +115,7 @@ def fp4_kv_read(pages: Tensor, slots: Tensor, *, head_dim: int,
                 dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
     """The K and V rows (N, kv_heads, head_dim) at ``slots`` (N,) int64 in ``dtype``; -1 gives zeros."""
     if backend.native_for(pages):
-        from saint_llm_b200.ops.gemm import error_word
-
-        k = torch.empty(slots.shape[0], pages.shape[1], head_dim, dtype=dtype, device=pages.device)
-        v = torch.empty_like(k)
-        backend.ext().fp4_kv_read(pages, slots, k, v, error_word(pages.device))
-        return k, v
+        return backend.ext().fp4_kv_read(pages, slots, head_dim, dtype, error_word(pages.device))
     if dtype not in _ROW_TYPES:
         raise ValueError("rows are read in bf16, fp16 or fp32")
     rows = fp4_kv_page_rows(pages, head_dim)
@@ -189,8 +183,6 @@ def fp4_kv_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, *
     if one:
         q = q.unsqueeze(2)
     if backend.native_for(q):
-        from saint_llm_b200.ops.gemm import error_word
-
         out = backend.ext().fp4_kv_attention(
             q, pages, table, lengths, window,
             sink if sink is None or sink.dtype == torch.float32 else sink.float(), float(softcap or 0.0),

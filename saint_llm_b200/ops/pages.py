@@ -17,6 +17,7 @@ import torch
 from torch import Tensor
 
 from saint_llm_b200.ops import backend
+from saint_llm_b200.ops.gemm import error_word
 
 
 def _check(pool: Tensor, table: Tensor, refcount: Tensor) -> None:
@@ -42,8 +43,6 @@ def fork_pages(pool: Tensor, table: Tensor, lengths: Tensor, refcount: Tensor, p
     the next one.  With too few free pages nothing changes, and an error is raised (on CUDA: by
     ``check_errors``).  Returns (table, lengths, refcount)."""
     if backend.native_for(pool):
-        from saint_llm_b200.ops.gemm import error_word
-
         return backend.ext().fork_pages(pool, table, lengths, refcount, parents, children, page_rows,
                                         error_word(pool.device))
     from saint_llm_b200.infer.paged_kv import PoolExhausted
@@ -88,8 +87,6 @@ def compact_pages(pool: Tensor, table: Tensor, refcount: Tensor) -> tuple[Tensor
     of a page that is not in use becomes -1).  Returns (table, refcount, n): afterwards the pages
     n and up are free.  Contents of pages that are free afterwards are unspecified."""
     if backend.native_for(pool):
-        from saint_llm_b200.ops.gemm import error_word
-
         return backend.ext().compact_pages(pool, table, refcount, error_word(pool.device))
     _check(pool, table, refcount)
     used = refcount > 0
