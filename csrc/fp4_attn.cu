@@ -23,25 +23,23 @@
 // * Operand order: dims and keys may be summed in any order, so a thread's operands are chosen to
 //   lie together: d/4 dims of a key for K; for V the d/16 bytes of its d/8 output dims, two keys'
 //   nibbles merged into the bytes that cvt turns into a pair.
-#include "fp4_kv.cuh"
-
-#include <algorithm>
-
-#include "common.cuh"
+#include "fp4_work.cuh"
 
 namespace sv4 {
 namespace {
+
+using namespace fp4;
 
 constexpr int kWarps = 4;
 constexpr int kTile = 32;  // keys per warp step
 // What a segment costs a block beside its tiles (queries, first copies, join), in tiles: with 8 blocks
 // that begin many short segments come last (prefill chunk 207 us, 176 with 16, 182 with 28).
 constexpr int kSegmentCost = 16;
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, int NT>
 struct Cfg {
-  static constexpr int kRows = 8 * NT;         // query rows of a segment
+  static constexpr int kRows = 8 * NT;  // query rows of a segment
+  using List = Work<kTile, kSegmentCost, kRows, kWarps>;
   static constexpr int kC = D / 32;            // scale blocks per row
   static constexpr int kCode = kTile * D / 2;  // bytes of K (or V) codes per stage
   static constexpr int kScale = kTile * kC;
@@ -65,25 +63,10 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Four bytes of two codes each -> four fp16 pairs (low code in the low half).
-__device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t (&o)[4]) {
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "mov.b32 {a, b, c, d}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(w));
-}
 // The low four bits of every byte from a, the high ones from b.
 __device__ __forceinline__ uint32_t low_nibbles_of(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("lop3.b32 %0, %1, %2, %3, 0xca;" : "=r"(d) : "r"(0x0f0f0f0fu), "r"(a), "r"(b));  // mask ? a : b
-  return d;
-}
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -98,60 +81,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
-// 2^(a - b) for a <= b, both possibly -inf
-__device__ __forceinline__ float shrink(float a, float b) { return a == b ? 1.f : ex2(a - b); }
-
-__device__ __forceinline__ float2 two_floats(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
-__device__ __forceinline__ float2 two_floats(uint32_t w, __nv_bfloat16) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-
-template <typename T, int N>
-struct alignas(sizeof(T) * N) Few {
-  T v[N];
-};
-
-// What the keys keep of the whole when a sink logit joins the denominator: their maximum is `top`
-// (log2 units) and their sum of p (times 2^15) is l.
-__device__ __forceinline__ float share_beside(float sink, float top, float l) {
-  if (l == 0.f) return 0.f;  // no key
-  const float s2 = sink * kLog2e;
-  if (s2 <= top) return l / (l + ex2(s2 - top + 15.f));
-  const float mine = l * ex2(top - s2);
-  return mine / (mine + 32768.f);
-}
-
-// Extremes of the scale bytes of the tile's rows (NaN blocks and zero blocks, bytes 0 and 1, left out).
-__device__ __forceinline__ void scale_range(uint32_t word, int n, int& lo, int& hi, bool& nan) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i >= n) break;
-    const int b = (word >> (8 * i)) & 255;
-    if (b == 255) nan = true;
-    else if (b > 1) {
-      lo = min(lo, b);
-      hi = max(hi, b);
-    }
-  }
-}
-
-// fp16 bits of 2^(byte - bias - 15) for bytes in (bias, bias + 28], else 0.
-__device__ __forceinline__ uint32_t scale_bits(int byte, int bias) {
-  const uint32_t f = static_cast<uint32_t>(byte - bias);
-  return f <= 28u ? f << 10 : 0u;
-}
-
 // The sums' unit moved from 2^from to 2^to: exact but for what leaves fp32's range at the small
 // end.  Towards smaller units only as far as the largest sum stays finite; returns the unit.
 template <int N, int NT>
@@ -175,53 +104,6 @@ __device__ __forceinline__ int to_unit(float (&acc)[N][NT][4], int from, int to)
   return from - up;
 }
 
-// The work as one list: for every sequence b, `row_tiles` (K / V head, 8 NT query rows) segments
-// of kSegmentCost + tiles(b) units each, the last tiles(b) of them key tiles.  Block i of the grid
-// takes the units [i per, (i + 1) per), so blocks have equal work whatever the lengths; a segment
-// whose tiles lie in several blocks is joined by the second kernel.  tiles(b) spans what any of
-// the T tokens may see.
-struct Span {
-  int len, start, tiles;  // sequence length, the tile boundary at or before the first key that anyone sees
-};
-
-__device__ __forceinline__ Span span_of(const Fp4AttnArgs& a, int b) {
-  Span s;
-  s.len = min(max(0, a.lengths[b]), a.P * a.R);
-  const int first = a.window > 0 ? max(0, s.len - a.T + 1 - a.window) : 0;
-  s.start = first & ~(a.R % kTile == 0 ? kTile - 1 : 15);
-  s.tiles = s.len > 0 ? (s.len - s.start + kTile - 1) / kTile : 0;
-  return s;
-}
-__device__ __forceinline__ int units_of(const Span& s) { return s.tiles > 0 ? s.tiles + kSegmentCost : 0; }
-
-// Sum of a segment's units for b < upto and over all b, by the whole block (every thread gets both).
-__device__ __forceinline__ void count_units(const Fp4AttnArgs& a, int upto, int& before, int& all) {
-  __shared__ int part[2][32];
-  int mine = 0, below = 0;
-  for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
-    const int n = units_of(span_of(a, b));
-    mine += n;
-    if (b < upto) below += n;
-  }
-  mine = __reduce_add_sync(0xffffffffu, mine);
-  below = __reduce_add_sync(0xffffffffu, below);
-  if ((threadIdx.x & 31) == 0) {
-    part[0][threadIdx.x >> 5] = below;
-    part[1][threadIdx.x >> 5] = mine;
-  }
-  __syncthreads();
-  before = all = 0;
-  for (int w = 0; w < static_cast<int>(blockDim.x + 31) / 32; ++w) {
-    before += part[0][w];
-    all += part[1][w];
-  }
-}
-
-// Units per block: at least one tile for each warp.
-__device__ __forceinline__ int units_per_block(const Fp4AttnArgs& a, int total) {
-  return max(kWarps, static_cast<int>((static_cast<uint32_t>(total) + a.blocks - 1) / a.blocks));
-}
-
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_rows_kernel(const Fp4AttnArgs a) {
   using C = Cfg<D, NT>;
@@ -241,39 +123,14 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
   const int64_t scale_src = static_cast<int64_t>(a.R) * D + scale_kv * a.R * C::kC + lane % C::kC * 16;
 
   // ---- this block's part of the list
-  int ignored, total;
-  count_units(a, 0, ignored, total);
-  total *= row_tiles;
-  const int per = units_per_block(a, total);
-  if (static_cast<int64_t>(blockIdx.x) * per >= total) return;
-  int skip = blockIdx.x * per, left = min(total - skip, per), b = 0;  // skip: into the sequences from b on
-  while (true) {  // 32 sequences at a time
-    const int n = b + lane < a.B ? units_of(span_of(a, b + lane)) * row_tiles : 0;
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    const uint32_t past = __ballot_sync(0xffffffffu, skip < upto);
-    if (past != 0) {
-      const int here = __ffs(past) - 1;
-      skip -= __shfl_sync(0xffffffffu, upto - n, here);
-      b += here;
-      break;
-    }
-    skip -= __shfl_sync(0xffffffffu, upto, 31);
-    b += 32;
-  }
-  Span sp = span_of(a, b);
-  int y = skip / units_of(sp), from_unit = skip - y * units_of(sp);
+  typename C::List list;
+  if (!list.begin(a, row_tiles)) return;
   // the scale's sign (or zero) goes into q; softcap works on natural units
   const float nat = (a.scale != 0.f ? fabsf(a.scale) : 1.f) * (a.softcap > 0.f ? 1.f : kLog2e);
 
   while (true) {
-    const int units = min(left, units_of(sp) - from_unit);
-    const int from_tile = max(0, from_unit - kSegmentCost);
-    const int take = from_unit + units - kSegmentCost - from_tile;  // may be 0 or less: only the segment's cost
+    const int take = list.take(), from_tile = list.from_tile(), b = list.b, y = list.y;
+    const Span sp = list.sp;
     if (take > 0) {
       const int head = y / tiles_per_head, row0 = (y % tiles_per_head) * C::kRows;
       const int rows = min(C::kRows, G * a.T - row0);
@@ -751,11 +608,10 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
         }
       }
       __syncthreads();
-      // This warp's part of the dim groups, of all warps' sums: the result if the whole segment is here,
-      // else part 0 (it began in an earlier block) or 1 (its first tile is here) of this block.
+      // This warp's part of the dim groups, of all warps' sums: the result, or a part of it.
       constexpr int kX = D >= 64 ? D / 64 : 1;
-      const bool whole = from_tile == 0 && take == sp.tiles;
-      const int64_t slot = (blockIdx.x * 2 + (from_tile == 0 ? 1 : 0)) * static_cast<int64_t>(C::kRows);
+      const bool whole = list.whole();
+      const int64_t slot = list.part_row();
       if (warp * kX < D / 16) {
 #pragma unroll
         for (int z = 0; z < NT; ++z) {
@@ -794,150 +650,44 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
     }
 
     // ---- the next segment
-    left -= units;
-    if (left == 0) return;
-    from_unit = 0;
-    if (++y == row_tiles) {
-      y = 0;
-      do sp = span_of(a, ++b);
-      while (sp.tiles == 0);
-    }
+    if (!list.next(a, row_tiles)) return;
     __syncthreads();  // the join's sums have been read
   }
-}
-
-// Joins the parts of a segment's rows, always in the same order; a segment that one block had whole
-// is done, one without keys is zero.  A block takes kRowsHere rows, so that each has 8 / kRowsHere
-// warps for its parts: one row where a segment may be cut into many parts, eight where into few.
-constexpr int kJoinWarps = 8;
-
-template <typename T, int D, int NT, int kRowsHere>
-__global__ void __launch_bounds__(kJoinWarps * 32) fp4_attn_join_kernel(const Fp4AttnArgs a) {
-  constexpr int kX = D / 32, kRows = Cfg<D, NT>::kRows, kDeep = kJoinWarps / kRowsHere;
-  __shared__ float sum[kJoinWarps][D];
-  __shared__ float2 ml[kJoinWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, deep = warp % kDeep;
-  const int G = a.H / a.Hk;
-  const int tiles_per_head = (G * a.T + kRows - 1) / kRows, row_tiles = a.Hk * tiles_per_head;
-  constexpr int kPerSegment = kRows / kRowsHere;
-  const int in_tile = blockIdx.x % kPerSegment * kRowsHere + warp / kDeep;
-  const int seg = blockIdx.x / kPerSegment, b = seg / row_tiles, y = seg - b * row_tiles;
-  const int i = (y % tiles_per_head) * kRows + in_tile;  // query row of the head
-  const int h = y / tiles_per_head * G + i % G;
-
-  int before, total;
-  count_units(a, b, before, total);
-  if (threadIdx.x == 0 && a.lengths[b] > a.P * a.R) record_error(a.err, kErrBounds);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Span sp = span_of(a, b);
-  T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.H + h) * a.T + i / G) * D + lane * kX;
-  const bool here = i < G * a.T;
-  if (sp.tiles == 0) {
-    Few<T, kX> zero;
-#pragma unroll
-    for (int d = 0; d < kX; ++d) zero.v[d] = static_cast<T>(0.f);
-    if (here && deep == 0) *reinterpret_cast<Few<T, kX>*>(out) = zero;
-    return;
-  }
-  const int per = units_per_block(a, total * row_tiles);
-  const int begin = before * row_tiles + y * units_of(sp) + kSegmentCost;  // its first tile
-  const int block0 = begin / per, block1 = (begin + sp.tiles - 1) / per;
-  if (block0 == block1) return;
-
-  float top = -INFINITY, l = 0.f, o[kX] = {};
-  if (here) {
-#pragma unroll 4
-    for (int x = block0 + deep; x <= block1; x += kDeep) {
-      // only the first can have begun at or behind its block's first unit
-      const int64_t slot = (static_cast<int64_t>(x) * 2 + (x == block0 && begin >= x * per ? 1 : 0)) * kRows + in_tile;
-      const float2 p = a.part_ml[slot];
-      const Few<float, kX> v = *reinterpret_cast<const Few<float, kX>*>(a.part_out + slot * D + lane * kX);
-      const float next = fmaxf(top, p.x);
-      const float keep = l * shrink(top, next), add = p.y * shrink(p.x, next);  // a part without keys adds 0
-      top = next;
-      l = keep + add;
-      const float old = l == 0.f ? 0.f : keep / l, now = l == 0.f ? 0.f : add / l;  // o is the mean so far
-#pragma unroll
-      for (int d = 0; d < kX; ++d) o[d] = o[d] * old + v.v[d] * now;
-    }
-  }
-  if constexpr (kDeep > 1) {
-#pragma unroll
-    for (int d = 0; d < kX; ++d) sum[warp][lane * kX + d] = o[d];
-    if (lane == 0) ml[warp] = make_float2(top, l);
-    __syncthreads();
-    if (deep != 0) return;
-    for (int w = warp + 1; w < warp + kDeep; ++w) {
-      const float2 p = ml[w];
-      const float next = fmaxf(top, p.x);
-      const float keep = l * shrink(top, next), add = p.y * shrink(p.x, next);
-      top = next;
-      l = keep + add;
-      const float old = l == 0.f ? 0.f : keep / l, now = l == 0.f ? 0.f : add / l;
-#pragma unroll
-      for (int d = 0; d < kX; ++d) o[d] = o[d] * old + sum[w][lane * kX + d] * now;
-    }
-  }
-  if (!here) return;
-  const float keep = a.sink != nullptr ? share_beside(a.sink[h], top, l) : 1.f;
-  Few<T, kX> r;
-#pragma unroll
-  for (int d = 0; d < kX; ++d) r.v[d] = static_cast<T>(o[d] * keep);
-  *reinterpret_cast<Few<T, kX>*>(out) = r;
 }
 
 template <typename T, int D, int NT>
 void launch(const Fp4AttnArgs& a, cudaStream_t stream) {
   using C = Cfg<D, NT>;
-  const int64_t segments = fp4_attn_segments(a);
   cudaFuncSetAttribute(fp4_attn_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   fp4_attn_rows_kernel<T, D, NT><<<a.blocks, kWarps * 32, C::kSmem, stream>>>(a);
-  // the join may start while the last blocks run: it waits where it reads their parts
-  cudaLaunchConfig_t join{};
-  // parts per segment: 16 or more take a block for each row (batch of 64: 1024 blocks 12 us, 128 blocks 6 us)
-  const bool deep = a.blocks >= 16 * segments;
-  join.gridDim = dim3(static_cast<unsigned>(segments * C::kRows / (deep ? 1 : 8)));
-  join.blockDim = dim3(kJoinWarps * 32);
-  join.stream = stream;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  join.attrs = &early;
-  join.numAttrs = 1;
-  if (deep) cudaLaunchKernelEx(&join, fp4_attn_join_kernel<T, D, NT, 1>, a);
-  else cudaLaunchKernelEx(&join, fp4_attn_join_kernel<T, D, NT, 8>, a);
+  launch_join<T, D, typename C::List>(a, stream);
 }
 
-template <typename T>
-void by_shape(const Fp4AttnArgs& a, int d, cudaStream_t stream) {
-  const bool few = fp4_attn_rows_per_segment(a) == 8;
-  if (d == 32) few ? launch<T, 32, 1>(a, stream) : launch<T, 32, 2>(a, stream);
-  else if (d == 64) few ? launch<T, 64, 1>(a, stream) : launch<T, 64, 2>(a, stream);
-  else few ? launch<T, 128, 1>(a, stream) : launch<T, 128, 2>(a, stream);
+// f(D, NT) for the head dim and the query rows of a K / V head: eight or fewer take 8-row segments
+// (2 x 131072 keys of 8 heads, 4 rows: 71 us, with 16-row segments 97).
+template <typename F>
+auto by_shape(const Fp4AttnArgs& a, int d, F&& f) {
+  using std::integral_constant;
+  const bool few = a.H / a.Hk * a.T <= 8;
+  if (d == 32) return few ? f(integral_constant<int, 32>{}, integral_constant<int, 1>{}) : f(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+  if (d == 64) return few ? f(integral_constant<int, 64>{}, integral_constant<int, 1>{}) : f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  return few ? f(integral_constant<int, 128>{}, integral_constant<int, 1>{}) : f(integral_constant<int, 128>{}, integral_constant<int, 2>{});
 }
 
 }  // namespace
 
-int fp4_attn_rows_per_segment(const Fp4AttnArgs& a) { return a.H / a.Hk * a.T <= 8 ? 8 : 16; }
-
-int64_t fp4_attn_segments(const Fp4AttnArgs& a) {
-  const int rows = fp4_attn_rows_per_segment(a);
-  return static_cast<int64_t>(a.B) * a.Hk * ((static_cast<int64_t>(a.H / a.Hk) * a.T + rows - 1) / rows);
-}
-
-int64_t fp4_attn_units(const Fp4AttnArgs& a) {
-  const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.P) * a.R, a.window > 0 ? static_cast<int64_t>(a.window) + a.T + 31 : INT32_MAX);
-  return fp4_attn_segments(a) * ((keys + kTile - 1) / kTile + kSegmentCost);
-}
-
-int fp4_attn_blocks(const Fp4AttnArgs& a, int d) {
-  const int64_t wave = 148 * (d == 128 && fp4_attn_rows_per_segment(a) == 16 ? 2 : 4);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wave, (fp4_attn_units(a) + kWarps - 1) / kWarps)));
+Fp4AttnPlan fp4_attn_rows_plan(const Fp4AttnArgs& a, int d) {
+  return by_shape(a, d, [&](auto dim, auto nt) {
+    using C = Cfg<decltype(dim)::value, decltype(nt)::value>;
+    return Fp4AttnPlan{C::List::most_units(a), C::List::blocks(a, C::kBlocks), C::kRows};
+  });
 }
 
 void fp4_attn_rows(const Fp4AttnArgs& a, int d, bool half, cudaStream_t stream) {
-  if (half) by_shape<__half>(a, d, stream);
-  else by_shape<__nv_bfloat16>(a, d, stream);
+  by_shape(a, d, [&](auto dim, auto nt) {
+    if (half) launch<__half, decltype(dim)::value, decltype(nt)::value>(a, stream);
+    else launch<__nv_bfloat16, decltype(dim)::value, decltype(nt)::value>(a, stream);
+  });
 }
 
 }  // namespace sv4

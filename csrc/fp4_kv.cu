@@ -231,6 +231,8 @@ torch::Tensor rows_aligned(const torch::Tensor& t) {
   return ok ? t : t.contiguous();
 }
 
+constexpr int kTileRows = 64;
+
 RowsArgs rows_args(const torch::Tensor& pages, const torch::Tensor& slots, int64_t d, const char* who) {
   RowsArgs a{};
   a.R = page_rows_of(pages, d, who);
@@ -363,13 +365,15 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   a.softcap = static_cast<float>(softcap);
   a.err = err.data_ptr<int>();
   TORCH_CHECK(B <= 65535 && H * T <= (1 << 26), "fp4_kv_attention: at most 65535 sequences and 2^26 query rows in each");
-  TORCH_CHECK(fp4_attn_units(a) < INT32_MAX, "fp4_kv_attention: more than 2^31 tiles of work in one call");
-  a.blocks = fp4_attn_blocks(a, static_cast<int>(d));
-  const int64_t part_rows = static_cast<int64_t>(a.blocks) * 2 * fp4_attn_rows_per_segment(a);
+  const bool many = d >= 64 && H / Hk * T >= kTileRows;
+  const Fp4AttnPlan plan = many ? fp4_attn_tile_plan(a) : fp4_attn_rows_plan(a, static_cast<int>(d));
+  TORCH_CHECK(plan.units < INT32_MAX, "fp4_kv_attention: more than 2^31 tiles of work in one call");
+  a.blocks = plan.blocks;
+  const int64_t part_rows = static_cast<int64_t>(plan.blocks) * 2 * plan.rows;
   torch::Tensor parts = uninitialised({part_rows * (d + 2)}, at::kFloat, q);
   a.part_ml = reinterpret_cast<float2*>(parts.data_ptr<float>());
   a.part_out = parts.data_ptr<float>() + 2 * part_rows;
-  fp4_attn_rows(a, static_cast<int>(d), q.scalar_type() == at::kHalf, at::cuda::getCurrentCUDAStream());
+  (many ? fp4_attn_tile : fp4_attn_rows)(a, static_cast<int>(d), q.scalar_type() == at::kHalf, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return out;
 }

@@ -31,14 +31,18 @@ struct Fp4AttnArgs {
   int* err;
 };
 
-// Query rows (heads of a K / V head times tokens) of one segment of work, the number of segments
-// (sequence, K / V head, rows), a bound on the units of work in all, and the blocks of one wave.
-int fp4_attn_rows_per_segment(const Fp4AttnArgs& a);
-int64_t fp4_attn_segments(const Fp4AttnArgs& a);
-int64_t fp4_attn_units(const Fp4AttnArgs& a);
-int fp4_attn_blocks(const Fp4AttnArgs& a, int d);
+// How a kernel divides the work: a bound on its units, the blocks of its grid, the rows of a part.
+struct Fp4AttnPlan {
+  int64_t units;
+  int blocks, rows;
+};
 
-// Launch for head_dim d (32, 64, 128) and q in fp16 or bf16.
+// Few query rows per K / V head: head_dim d (32, 64, 128), q in fp16 or bf16.
+Fp4AttnPlan fp4_attn_rows_plan(const Fp4AttnArgs& a, int d);
 void fp4_attn_rows(const Fp4AttnArgs& a, int d, bool half, cudaStream_t stream);
+
+// Many: head_dim 64 or 128.
+Fp4AttnPlan fp4_attn_tile_plan(const Fp4AttnArgs& a);
+void fp4_attn_tile(const Fp4AttnArgs& a, int d, bool half, cudaStream_t stream);
 
 }  // namespace sv4

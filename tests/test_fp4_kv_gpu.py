@@ -81,6 +81,64 @@ def test_attention_long_cache_in_splits(cuda):
     _attend_case(cuda, [9001], h=4, hk=4, d=64, rows=128, dtype=torch.float16)
 
 
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_attention_of_many_rows(cuda, d, dtype):
+    """64 query rows per K / V head and more: the tensor-core tiles, at their edges."""
+    _attend_case(cuda, [128, 129, 300, 0, 39, 1], h=4, hk=2, d=d, rows=16, t=40, dtype=dtype, sink=True)
+    _attend_case(cuda, [700, 256], h=3, hk=1, d=d, rows=48, t=70, dtype=dtype, softcap=12.0, qscale=3.0)
+    _attend_case(cuda, [513, 140], h=16, hk=1, d=d, rows=64, t=9, dtype=dtype, window=100, sink=True)
+    _attend_case(cuda, [3000], h=64, hk=1, d=d, rows=128, t=2, dtype=dtype)
+
+
+@pytest.mark.parametrize("spread", [6, 30, 55])
+def test_attention_of_many_rows_of_very_different_size(cuda, spread):
+    _attend_case(cuda, [5, 64, 333], h=8, hk=1, d=128, rows=32, t=16, spread=spread, qscale=8.0)
+    _attend_case(cuda, [260], h=8, hk=2, d=64, rows=16, t=33, spread=spread, qscale=30.0)
+
+
+def test_attention_of_many_rows_sharp_scores(cuda):
+    _attend_case(cuda, [300, 200], h=8, hk=1, d=128, rows=64, t=20, qscale=60.0)
+    _attend_case(cuda, [300], h=8, hk=1, d=64, rows=64, t=20, qscale=0.0)
+    _attend_case(cuda, [300], h=8, hk=1, d=128, rows=64, t=20, qscale=2.0 ** 60, one_hot=True)
+
+
+def test_attention_of_many_rows_nan_and_bad_pages(cuda):
+    from saint_llm_b200.ops.fp4_kv import fp4_kv_attention, fp4_kv_write
+    from saint_llm_b200.ops.gemm import check_errors
+
+    gen = torch.Generator().manual_seed(11)
+    pages, table, lengths = oracle.filled([200, 180], hk=1, d=128, rows=16, gen=gen, device=cuda)
+    q = torch.randn(2, 8, 30, 128, generator=gen).to(cuda, torch.bfloat16)
+    clean = fp4_kv_attention(q, pages, table, lengths)
+    for which in range(2):
+        k, v = torch.randn(2, 1, 1, 128, generator=gen).to(cuda).unbind(0)
+        (k, v)[which][0, 0, 40] = float("inf")
+        mine = pages.clone()
+        fp4_kv_write(k, v, mine, table[0, 195 // 16].long().view(1) * 16 + 195 % 16)  # queries 25 .. 29 see key 195
+        got = fp4_kv_attention(q, mine, table, lengths)
+        assert bool(got[0, :, 25:].isnan().all() if which == 0 else got[0, :, 25:, 32:64].isnan().all())
+        assert torch.equal(got[1], clean[1]) and torch.equal(got[0, :, :25], clean[0, :, :25])
+        if which == 1:
+            assert bool(got[0, :, 25:, :32].isfinite().all() and got[0, :, 25:, 64:].isfinite().all())
+    broken = table.clone()
+    broken[0, 3] = 10 ** 6
+    out = fp4_kv_attention(q, pages, broken, lengths)
+    with pytest.raises(RuntimeError, match="out of bounds"):
+        check_errors(cuda)
+    assert bool(out.isfinite().all()) and torch.equal(out[1], clean[1])
+    # without the keys of that page: the same as a cache in which they were never there
+    keep = [i for i in range(200) if i // 16 != 3]
+    gathered = torch.zeros_like(pages)
+    from saint_llm_b200.ops.fp4_kv import fp4_kv_read
+
+    slots = table[0, torch.tensor(keep, device=cuda) // 16].long() * 16 + torch.tensor(keep, device=cuda) % 16
+    k, v = fp4_kv_read(pages, slots, head_dim=128, dtype=torch.float32)
+    fp4_kv_write(k, v, gathered, torch.arange(len(keep), device=cuda))
+    ids = torch.arange(12, dtype=torch.int32, device=cuda).view(1, 12)
+    want, size, score, floor = oracle.attention(q[:1], gathered, ids, torch.tensor([len(keep)], device=cuda), 16)
+    assert bool(((out[:1].double() - want).abs() <= oracle.bound(want, size, score, floor, q.dtype)).all())
+
+
 def test_attention_nan_reaches_only_the_rows_that_see_it(cuda):
     from saint_llm_b200.ops.fp4_kv import fp4_kv_attention, fp4_kv_write
 
