@@ -3,18 +3,22 @@
 //
 // The mathematics, the list of work and the join are those of fp4_attn.cu.  Here 4 * 128 * 128 * d
 // operations per tile stand against 128 * 17/16 d bytes, so the tensor cores bound it, and next to
-// them the exponentials (128 * 128 per tile, 16 a clock) and the turning of codes into operands:
+// them the exponentials (128 * 128 per tile, 16 a clock) and the turning of codes into operands.
+// A block has two roles, two blocks share an SM:
 //
-// * A block has 128 threads and one 128-row tile of queries (the G heads of a K / V head, times
-//   tokens); thread = row = TMEM lane.  Two blocks per SM, one's products under the other's
-//   softmax.  S and O accumulate in TMEM (fp32), the operands lie in shared memory as 64-column
-//   128B-swizzled atoms, V contracted over its rows; P takes K's place.
-// * Codes go from global memory to registers a tile ahead (eight rows of one 32-value block per
-//   eight threads: coalesced reads, conflict-free swizzled writes), through cvt.e2m1x2 to fp16,
-//   exact, times their scale 2^e, exact for exponents in [-14, 13].  V is written while S = Q K^T runs.
-// * A tile with other exponents takes K's from its own largest 28 down, and runs P V once per window
-//   of 28 exponents, each row's sums moved from unit to unit by powers of two; a row whose sums are
-//   too large to follow to a small unit has no use for what is 2^-126 of them.
+// * Warps 0 - 3, the softmax of a 128-row tile of queries (the G heads of a K / V head, times
+//   tokens): thread = row = TMEM lane.  S is read from TMEM, P (fp16, times 2^15) written over it as
+//   the A operand of P V; O accumulates in TMEM too.  A row's maximum is left as it is while the new
+//   one is at most 0.9 larger (log2), for which fp16 has room: most tiles then leave O alone.
+//   One thread issues the products.
+// * Warps 4 - 7, operands: codes from global memory to registers a tile ahead (eight rows of one
+//   32-value block per eight threads: coalesced reads, conflict-free swizzled writes), through
+//   cvt.e2m1x2 to fp16, exact, times their scale 2^e, exact for exponents in [-14, 13].  K and V lie
+//   as 64-column 128B-swizzled atoms, V contracted over its rows.
+//
+// A tile with other exponents takes K's from its own largest 28 down, and runs P V once per window
+// of 28 exponents, each row's sums moved from unit to unit by powers of two; a row whose sums are
+// too large to follow to a small unit has no use for what is 2^-126 of them.
 #include "fp4_work.cuh"
 
 namespace sv4 {
@@ -22,54 +26,129 @@ namespace {
 
 using namespace fp4;
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
 constexpr int kKeys = 128, kRows = 128;
 constexpr int kSegmentCost = 4;       // in tiles
 constexpr uint32_t kAtom = 16384;     // 128 rows x 128 bytes
+constexpr int kWindows = 10;          // 28 exponents each
 using List = Work<kKeys, kSegmentCost, kRows, 1>;
 
-// Operand descriptors: contraction over columns (step s of 16), over rows.
-__device__ __forceinline__ uint64_t desc_cols(uint32_t base, int s) {
-  return make_smem_desc(base + (s >> 2) * kAtom + (s & 3) * 32, 16, 1024, 2);
-}
-__device__ __forceinline__ uint64_t desc_rows(uint32_t base, int s) {
-  return make_smem_desc(base + s * 2048, kAtom, 1024, 2);
-}
-// Where 16-byte piece q (of the 64-column atom's eight) of row r lies.
+// Operand descriptors, contracted over columns or over rows, and how far step s of 16 is from the
+// first (the address field counts 16 bytes, and no step leaves it).
+__device__ __forceinline__ uint64_t desc_cols(uint32_t base) { return make_smem_desc(base, 16, 1024, 2); }
+__device__ __forceinline__ uint64_t desc_rows(uint32_t base) { return make_smem_desc(base, kAtom, 1024, 2); }
+constexpr uint32_t step_cols(int s) { return ((s >> 2) * kAtom + (s & 3) * 32) >> 4; }
+constexpr uint32_t step_rows(int s) { return s * 2048 >> 4; }
+// Where the 16-byte piece of `column` (a multiple of 8) of row r lies.
 __device__ __forceinline__ uint8_t* piece_at(uint8_t* tile, int r, int column) {
   return tile + (column >> 6) * kAtom + r * 128 + ((((column & 63) >> 3) ^ (r & 7)) << 4);
 }
+// D += A B with A (fp16 pairs, a row per lane) in TMEM.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// What the operand warps say about a tile.
+struct Tile {
+  int plain;   // all exponents in [-14, 13] and every page there
+  int kbias;   // K's scales are 2^(byte - kbias - 15)
+  int windows; // products P V
+  int bias[kWindows];
+  uint32_t nan_keys[kKeys];  // bits 0 - 3: blocks of V that are NaN; bit 31: a key whose page id is bad
+};
 
 template <int D>
 struct Cfg {
   static constexpr int kAtoms = D / 64;
-  static constexpr int kQ = kAtoms * kAtom, kKP = 2 * kAtom, kV = kAtoms * kAtom;  // P: two atoms whatever D
-  // alignment, barriers and flags; as much for every D, so that two blocks' TMEM is all an SM is asked for
-  static constexpr int kSmem = 6 * kAtom + 1024 + 1024;
+  static constexpr int kQ = kAtoms * kAtom;
   static constexpr int kC = D / 32;
-  static constexpr int kRowsAtOnce = 32 / kC;         // a warp's rows per pass: lane = (block, row)
-  static constexpr int kPasses = 32 / kRowsAtOnce;    // a warp writes 32 rows
+  static constexpr int kRowsAtOnce = 32 / kC;       // a warp's rows per pass: lane = (block, row)
+  static constexpr int kPasses = 32 / kRowsAtOnce;  // a warp writes 32 rows
+  // q, K, V, alignment, barriers and tiles; as much for every D, so that two blocks' TMEM is all an SM is asked for
+  static constexpr int kSmem = 6 * kAtom + 1024 + 2048;
 };
+
+// The largest v over the four operand warps.
+__device__ __forceinline__ int most_of(int v, int* red, int part, int lane) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  if (lane == 0) red[part] = v;
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  return max(max(red[0], red[1]), max(red[2], red[3]));
+}
+
+// A tile with exponents outside [-14, 13], NaN blocks or missing keys: K's bias, V's windows and the
+// keys' marks, from the scale bytes (one per pass) of all operand threads.  Returns {kbias, windows}.
+// Not inlined: its registers would be taken from every tile.
+template <int D>
+__device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uint32_t vbytes, uint32_t seen, uint32_t lost,
+                                      int part, int lane) {
+  using C = Cfg<D>;
+  const int in_row = lane % C::kRowsAtOnce, blk = lane / C::kRowsAtOnce;
+  int khi = 0, vhi = 0;
+  for (int x = 0; x < C::kPasses; ++x) {
+    if (!((seen >> x) & 1u)) continue;
+    const int k = (kbytes >> (8 * x)) & 255u, v = (vbytes >> (8 * x)) & 255u;
+    if (k != 255) khi = max(khi, k);
+    if (v != 255) vhi = max(vhi, v);
+  }
+  const int kbias = max(most_of(khi, red, part, lane) - 28, -14);
+  int bias = max(most_of(vhi, red, part, lane) - 28, 2), windows = 1;
+  const bool scribe = part == 0 && lane == 0;
+  if (scribe) tile.bias[0] = bias;
+  while (windows < kWindows) {
+    int below = 0;  // the largest byte that no window holds yet
+    for (int x = 0; x < C::kPasses; ++x) {
+      const int v = (vbytes >> (8 * x)) & 255u;
+      if (((seen >> x) & 1u) && v <= bias && v > 1) below = max(below, v);
+    }
+    below = most_of(below, red, part, lane);
+    if (below == 0) break;
+    bias = below - 28;
+    if (scribe) tile.bias[windows] = bias;
+    ++windows;
+  }
+  tile.nan_keys[32 * part + lane] = 0;
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  for (int x = 0; x < C::kPasses; ++x) {
+    const int row = 32 * part + C::kRowsAtOnce * x + in_row;
+    if (((seen >> x) & 1u) && ((vbytes >> (8 * x)) & 255u) == 255u) atomicOr(tile.nan_keys + row, 1u << blk);
+    if ((lost >> x) & 1u) atomicOr(tile.nan_keys + row, 0x80000000u);
+  }
+  return make_int2(kbias, windows);
+}
+
+enum Barrier { kQFull, kKFull, kSFull, kPFull, kVFull, kOFull, kBarriers };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4AttnArgs a) {
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sq = smem, *sk = sq + C::kQ, *sv = sk + C::kKP, *sp = sk;
-  uint64_t* bar = reinterpret_cast<uint64_t*>(sv + C::kV);  // 0: S is there, 1: P V is done
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(bar + 2);
-  int* red = reinterpret_cast<int*>(tslot + 1);                // (4)
-  uint32_t* nan_keys = reinterpret_cast<uint32_t*>(red + 4);   // (128) blocks of V that are NaN
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t *sq = smem, *sk = sq + C::kQ, *sv = sk + C::kQ;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + 6 * kAtom);
+  Tile* tiles = reinterpret_cast<Tile*>(bar + kBarriers);  // (2), by turns
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(tiles + 2);
+  int* red = reinterpret_cast<int*>(tslot + 1);  // (4)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.H / a.Hk, tiles_per_head = (G * a.T + kRows - 1) / kRows, row_tiles = a.Hk * tiles_per_head;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   List list;
   if (!list.begin(a, row_tiles)) return;
-  if (tid == 0) {
-    mbar_init(bar, 1);
-    mbar_init(bar + 1, 1);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBarriers; ++i) mbar_init(bar + i, i == kSFull || i == kOFull ? 1 : 4);
     fence_barrier_init();
   }
   if (warp == 0) {
@@ -79,122 +158,189 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = *tslot, lanes = static_cast<uint32_t>(warp * 32) << 16;
-  const uint32_t ts = tbase + lanes, to = tbase + 128 + lanes;
-  constexpr uint32_t kIdS = make_idesc_f16(128, 128, 0, 0, false, false);
-  constexpr uint32_t kIdO = make_idesc_f16(128, D, 0, 0, false, true);
-  const uint32_t uq = smem_u32(sq), uk = smem_u32(sk), uv = smem_u32(sv), up_ = smem_u32(sp);
-  uint32_t n_s = 0, n_o = 0;  // products so far: parities of the two barriers
+  const uint32_t tbase = *tslot;
+  // The n-th completion of a barrier.  A wait that runs out records itself; the role then ends.
   bool alive = true;
   auto wait = [&](int which, uint32_t n) {
-    if (!mbar_wait(bar + which, n & 1, nullptr, 0)) {
+    if (alive && !mbar_wait(bar + which, n & 1, nullptr, 0)) {
       record_error(a.err, kErrTimeoutAccum);
       alive = false;
     }
     __syncwarp();
-    tc_fence_after();
   };
-  const float nat = (a.scale != 0.f ? fabsf(a.scale) : 1.f) * (a.softcap > 0.f ? 1.f : kLog2e);
-  const int in_row = lane % C::kRowsAtOnce, blk = lane / C::kRowsAtOnce;  // of a pass: row, 32-value block
+  auto arrive = [&](int which) {  // one per warp
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar + which);
+  };
+  // Every role counts the same: segments, tiles and P V products so far.
+  uint32_t n_seg = 0, n_tile = 0, n_pv = 0;
 
   while (true) {
     const int take = list.take(), from_tile = list.from_tile(), b = list.b;
-    if (take > 0) {
-      const int head = list.y / tiles_per_head, row0 = (list.y % tiles_per_head) * kRows;
-      const int rows = min(kRows, G * a.T - row0), len = list.sp.len;
-      auto end_of = [&](int i) { return len - a.T + (row0 + min(i, rows - 1)) / G + 1; };  // one past the last key of row i
-      const int hi = end_of(tid), lo = a.window > 0 ? max(0, hi - a.window) : 0;
-      const int last = end_of(kRows - 1), inner_hi = end_of(0);
-      const int first = a.window > 0 ? max(0, inner_hi - a.window) : 0, inner_lo = a.window > 0 ? max(0, last - a.window) : 0;
-      const int* table = a.table + static_cast<int64_t>(b) * a.P;
-      const int key_begin = list.sp.start + from_tile * kKeys;
+    const int head = list.y / tiles_per_head, row0 = (list.y % tiles_per_head) * kRows;
+    const int rows = min(kRows, G * a.T - row0), len = list.sp.len;
+    auto end_of = [&](int i) { return len - a.T + (row0 + min(i, rows - 1)) / G + 1; };  // one past the last key of row i
+    const int last = end_of(kRows - 1), inner_hi = end_of(0);
+    const int first = a.window > 0 ? max(0, inner_hi - a.window) : 0;
+    const int key_begin = list.sp.start + from_tile * kKeys;
+    // tiles behind what this row tile sees are left out (the list spans all T tokens)
+    const int count = take > 0 && key_begin < last ? min(take, (last - key_begin + kKeys - 1) / kKeys) : 0;
 
-      // ---- codes and scale bytes of a tile: pass x of this warp has rows 32 warp + kRowsAtOnce x + in_row
-      uint4 kcode[C::kPasses], vcode[C::kPasses];
-      uint32_t kbyte = 0, vbyte = 0;   // one byte per pass
-      uint32_t here = 0;               // passes whose row may be seen, of the tile that K is loaded for
-      uint32_t vhere = 0;
-      uint32_t lost = 0;               // passes whose page id is bad
-      const uint8_t* at[C::kPasses];   // the slab, or null, for the tile after
-      int at_row[C::kPasses];
+    if (warp >= 4) {
+      // ============================================================ operands
+      const int part = warp - 4, in_row = lane % C::kRowsAtOnce, blk = lane / C::kRowsAtOnce;
+      const int* table = a.table + static_cast<int64_t>(b) * a.P;
+      // Rows of a pass x: 32 part + kRowsAtOnce x + in_row of a tile.  A warp's 32 rows lie in one page if
+      // pages have multiples of 32 rows (tiles then start at one), else 16 by 16.
+      const bool one_page = a.R % 32 == 0;
+      int page[2] = {-1, -1}, in_page[2] = {0, 0};       // of the tile to load next: its 16-row halves
       auto find = [&](int key0) {
 #pragma unroll
-        for (int x = 0; x < C::kPasses; ++x) {
-          const int key = key0 + 32 * warp + C::kRowsAtOnce * x + in_row;
-          at[x] = nullptr;
-          at_row[x] = 0;
-          if (key < last) {
-            const int slot = key / a.R, page = table[slot];
-            if (index_ok(page, 0, a.n_pages, a.err)) {
-              at[x] = a.pages + page * a.page_stride + static_cast<int64_t>(head) * a.slab;
-              at_row[x] = key - slot * a.R;
-            }
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && one_page) {
+            page[1] = page[0];
+            in_page[1] = in_page[0] + 16;
+            break;
           }
+          const int key = key0 + 32 * part + 16 * h;
+          const int slot = key / a.R;
+          page[h] = key < last ? table[slot] : -2;  // -2: nobody sees it
+          in_page[h] = key - slot * a.R;
         }
       };
-      auto load = [&](uint4 (&code)[C::kPasses], uint32_t& bytes, int kv) {
-        bytes = 0;
+      // Loads without branches between them, so that all are in flight at once: a row that nobody may
+      // see, or whose page id is bad, is read from the pool's first page and left out where it is used.
+      uint4 code[C::kPasses];  // K's, then V's
+      uint8_t kraw[C::kPasses], vraw[C::kPasses];
+      uint32_t seen = 0, lost = 0;  // passes whose row may be seen; whose page id is bad
+      const uint8_t* rows_at[2];    // this thread's first K codes of each half
+      auto load_codes = [&](int64_t offset) {
 #pragma unroll
-        for (int x = 0; x < C::kPasses; ++x) {
-          code[x] = make_uint4(0, 0, 0, 0);
-          if (at[x] != nullptr) {
-            code[x] = *reinterpret_cast<const uint4*>(at[x] + (kv * a.R + at_row[x]) * (D / 2) + blk * 16);
-            bytes |= static_cast<uint32_t>(at[x][a.R * D + (kv * a.R + at_row[x]) * C::kC + blk]) << (8 * x);
+        for (int x = 0; x < C::kPasses; ++x)
+          code[x] = *reinterpret_cast<const uint4*>(rows_at[x / (C::kPasses / 2)] + offset +
+                                                    x % (C::kPasses / 2) * C::kRowsAtOnce * (D / 2));
+      };
+      auto load = [&](int key0) {
+        seen = lost = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bool wanted = page[h] != -2, ok = wanted && index_ok(page[h], 0, a.n_pages, a.err);
+          const uint8_t* slab = a.pages + (ok ? page[h] : 0) * a.page_stride + static_cast<int64_t>(head) * a.slab;
+          const int r = (ok ? in_page[h] : 0) + in_row;
+          const uint8_t* scales = slab + a.R * D + r * C::kC + blk;
+          rows_at[h] = slab + r * (D / 2) + blk * 16;
+#pragma unroll
+          for (int y = 0; y < C::kPasses / 2; ++y) {
+            const int x = h * (C::kPasses / 2) + y, key = key0 + 32 * part + C::kRowsAtOnce * x + in_row;
+            kraw[x] = scales[y * C::kRowsAtOnce * C::kC];
+            vraw[x] = scales[a.R * C::kC + y * C::kRowsAtOnce * C::kC];
+            if (key >= first && key < last) (ok ? seen : lost) |= 1u << x;
           }
         }
+        load_codes(0);
       };
-      auto seen_mask = [&](int key0) {
-        uint32_t m = 0, gone = 0;
+      // fp16 values of this thread's rows into a swizzled tile (at `offset` from K's); scale(x) gives the
+      // scale's fp16 bits.  A row's eight-row phase does not depend on the pass: four addresses do.
+      uint32_t to_piece[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) to_piece[q] = smem_u32(piece_at(sk, 32 * part + in_row, blk * 32 + q * 8));
+      auto write = [&](uint32_t offset, auto&& scale) {
 #pragma unroll
         for (int x = 0; x < C::kPasses; ++x) {
-          const int key = key0 + 32 * warp + C::kRowsAtOnce * x + in_row;
-          if (key >= first && key < last) {
-            if (at[x] != nullptr) m |= 1u << x;
-            else gone |= 1u << x;
-          }
-        }
-        lost = gone;
-        return m;
-      };
-      // fp16 values of this thread's rows into a swizzled tile; scale(byte) gives the scale's fp16 bits
-      auto write = [&](uint8_t* tile, const uint4 (&code)[C::kPasses], auto&& scale) {
-#pragma unroll
-        for (int x = 0; x < C::kPasses; ++x) {
-          const int row = 32 * warp + C::kRowsAtOnce * x + in_row;
           const uint32_t s = scale(x) * 0x10001u;
           const uint32_t w[4] = {code[x].x, code[x].y, code[x].z, code[x].w};
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t h[4];
             codes_to_half2(w[q], h);
-            *reinterpret_cast<uint4*>(piece_at(tile, row, blk * 32 + q * 8)) =
-                make_uint4(mul2(h[0], s), mul2(h[1], s), mul2(h[2], s), mul2(h[3], s));
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(to_piece[q] + offset + C::kRowsAtOnce * 128 * x), "r"(mul2(h[0], s)), "r"(mul2(h[1], s)),
+                           "r"(mul2(h[2], s)), "r"(mul2(h[3], s)) : "memory");
           }
         }
       };
-      auto byte_of = [](uint32_t bytes, int x) { return static_cast<int>((bytes >> (8 * x)) & 255u); };
-      auto block_max = [&](int v) {
-        v = __reduce_max_sync(0xffffffffu, v);
-        if (lane == 0) red[warp] = v;
-        __syncthreads();
-        v = max(max(red[0], red[1]), max(red[2], red[3]));
-        __syncthreads();
-        return v;
-      };
-
-      find(key_begin);
-      load(kcode, kbyte, 0);
-      load(vcode, vbyte, 1);
-
-      // ---- q: thread = row, scaled by a power of two to fp16's top, into the swizzled tile
-      float factor;  // raw score -> softmax units
-      {
-        const int i = row0 + min(tid, rows - 1);
-        const T* row = static_cast<const T*>(a.q) + b * a.q_b + (head * G + i % G) * a.q_h + (i / G) * a.q_t;
+      bool careful = false;  // a tile of this segment had other exponents: its sums have units
+      if (count > 0) {
+        find(key_begin);
+        load(key_begin);
+        find(key_begin + kKeys);
+      }
+      for (int t = 0; t < count && alive; ++t) {
+        const int key0 = key_begin + t * kKeys;
+        Tile& tile = tiles[n_tile & 1];
+        bool ok = lost == 0;
+#pragma unroll
+        for (int x = 0; x < C::kPasses; ++x) {
+          const int k = static_cast<int>(kraw[x]), v = static_cast<int>(vraw[x]);
+          // exponents [-14, 13], or a block of zeros
+          ok = ok && (!((seen >> x) & 1u) || ((k <= 1 || (k > 112 && k <= 140)) && (v <= 1 || (v > 112 && v <= 140))));
+        }
+        if (n_tile > 0) wait(kSFull, n_tile - 1);  // K is free
+        const bool plain = most_of(ok ? 0 : 1, red, part, lane) == 0 && !careful;
+        int kbias = 112, windows = 1;
+        const bool scribe = part == 0 && lane == 0;
+        if (!plain) {
+          careful = true;
+          uint32_t kbytes = 0, vbytes = 0;
+#pragma unroll
+          for (int x = 0; x < C::kPasses; ++x) {
+            kbytes |= static_cast<uint32_t>(kraw[x]) << (8 * x);
+            vbytes |= static_cast<uint32_t>(vraw[x]) << (8 * x);
+          }
+          const int2 found = describe<D>(tile, red, kbytes, vbytes, seen, lost, part, lane);
+          kbias = found.x;
+          windows = found.y;
+        }
+        if (scribe) {
+          tile.plain = plain;
+          tile.kbias = kbias;
+          tile.windows = windows;
+        }
+        write(0, [&](int x) {
+          const int k = static_cast<int>(kraw[x]);
+          return !((seen >> x) & 1u) ? 0u : k == 255 ? 0x7e00u : scale_bits(k, kbias);
+        });
+        load_codes(a.R * (D / 2));
+        fence_proxy_async_smem();
+        arrive(kKFull);
+        for (int w = 0; w < windows && alive; ++w) {
+          if (n_pv > 0) wait(kOFull, n_pv - 1);  // V is free
+          // (or the conversions, the same for all windows, would be kept in registers)
+#pragma unroll
+          for (int x = 0; x < C::kPasses; ++x) asm volatile("" : "+r"(code[x].x), "+r"(code[x].y), "+r"(code[x].z), "+r"(code[x].w));
+          const int least = plain ? 112 : tile.bias[w], most = w == 0 ? 254 : tile.bias[w - 1];
+          write(C::kQ, [&](int x) {
+            const int v = static_cast<int>(vraw[x]);
+            return !((seen >> x) & 1u) || v > most ? 0u : scale_bits(v, least);
+          });
+          fence_proxy_async_smem();
+          arrive(kVFull);
+          ++n_pv;
+        }
+        if (t + 1 < count) {
+          load(key0 + kKeys);
+          find(key0 + 2 * kKeys);
+        }
+        ++n_tile;
+      }
+    } else {
+      // ============================================================ softmax
+      constexpr uint32_t kIdS = make_idesc_f16(128, 128, 0, 0, false, false);
+      constexpr uint32_t kIdO = make_idesc_f16(128, D, 0, 0, false, true);
+      const uint64_t dq = desc_cols(smem_u32(sq)), dk = desc_cols(smem_u32(sk)), dv = desc_rows(smem_u32(sv));
+      const int row = threadIdx.x;  // of the tile; the warp's TMEM lanes
+      const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16, ts = tbase + lanes, to = tbase + 128 + lanes;
+      const int hi = end_of(row), lo = a.window > 0 ? max(0, hi - a.window) : 0;
+      const int inner_lo = a.window > 0 ? max(0, last - a.window) : 0;
+      const float nat = (a.scale != 0.f ? fabsf(a.scale) : 1.f) * (a.softcap > 0.f ? 1.f : kLog2e);
+      float factor = 0.f;  // raw score -> softmax units
+      if (count > 0) {
+        const int i = row0 + min(row, rows - 1);
+        const T* from = static_cast<const T*>(a.q) + b * a.q_b + (head * G + i % G) * a.q_h + (i / G) * a.q_t;
         float amax = 0.f;
 #pragma unroll 4
         for (int k = 0; k < D / 8; ++k) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(row + 8 * k);
+          const uint4 raw = *reinterpret_cast<const uint4*>(from + 8 * k);
           const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -203,12 +349,12 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           }
         }
         const int x = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-        const int up = amax > 0.f && x < 128 ? min(14 - x, 126) : 0;
+        const int up = amax > 0.f && x < 128 ? min(14 - x, 126) : 0;  // to fp16's top
         const float f = a.scale > 0.f ? pow2f(up) : a.scale < 0.f ? -pow2f(up) : 0.f;
         factor = pow2f(max(-up, -126)) * nat;
 #pragma unroll 4
         for (int k = 0; k < D / 8; ++k) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(row + 8 * k);
+          const uint4 raw = *reinterpret_cast<const uint4*>(from + 8 * k);
           const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
           uint32_t h[4];
 #pragma unroll
@@ -216,131 +362,101 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
             const float2 v = two_floats(w[y], T{});
             h[y] = pack_half2(v.x * f, v.y * f);
           }
-          *reinterpret_cast<uint4*>(piece_at(sq, tid, 8 * k)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(piece_at(sq, row, 8 * k)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
+        fence_proxy_async_smem();
+        arrive(kQFull);
+        if (warp == 0) wait(kQFull, n_seg);
       }
 
       float m = -INFINITY, l = 0.f;
-      int unit = 0;           // this row's sums are held times 2^-unit
-      uint32_t poison = 0;    // blocks of d whose sums are NaN
-      bool careful = false;   // units have moved: the block's tiles take the careful way
-      bool out_of_range = false;
-      uint32_t n_tile = 0;    // P V products of this segment
-
-      for (int t = 0; t < take && alive; ++t) {
+      int unit = 0;                // this row's sums are held times 2^-unit
+      uint32_t poison = 0;         // blocks of d whose sums are NaN
+      bool out_of_range = false;   // maxima above 2^16
+      auto each_sum = [&](auto&& change) {  // of this row in TMEM
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(to + c * 32, r);
+          tmem_ld_wait();
+          change(r);
+          tmem_st32(to + c * 32, r);
+        }
+        tmem_st_wait();
+      };
+      for (int t = 0; t < count && alive; ++t) {
         const int key0 = key_begin + t * kKeys;
-        if (key0 >= last) break;  // behind what this row tile sees (the list spans all T tokens)
-        here = seen_mask(key0);
-        vhere = here;
-        bool ok = lost == 0;
+        wait(kKFull, n_tile);  // the operand warps' word on the tile
+        if (warp == 0) {
+          if (n_pv > 0) wait(kOFull, n_pv - 1);  // P lies where S goes
+          if (alive && elect_one()) {
+            tc_fence_after();
 #pragma unroll
-        for (int x = 0; x < C::kPasses; ++x) {
-          const int k = byte_of(kbyte, x), v = byte_of(vbyte, x);
-          // exponents [-14, 13], or a block of zeros
-          ok = ok && (!((here >> x) & 1u) || ((k <= 1 || (k > 112 && k <= 140)) && (v <= 1 || (v > 112 && v <= 140))));
-        }
-        if (n_tile > 0) wait(1, n_o - 1);  // P V of the last tile: its operands are free
-        const bool plain = __syncthreads_and(ok) && !careful;
-        int kbias = 112, vbias = 112;
-        if (!plain) {
-          int khi = 0, vhi = 0;
-#pragma unroll
-          for (int x = 0; x < C::kPasses; ++x) {
-            if (!((here >> x) & 1u)) continue;
-            const int k = byte_of(kbyte, x), v = byte_of(vbyte, x);
-            if (k != 255) khi = max(khi, k);
-            if (v != 255) vhi = max(vhi, v);
+            for (int s = 0; s < D / 16; ++s) mma_bf16(tbase, dq + step_cols(s), dk + step_cols(s), kIdS, s > 0 ? 1u : 0u);
+            mma_commit(bar + kSFull);
           }
-          kbias = max(block_max(khi) - 28, -14);
-          vbias = max(block_max(vhi) - 28, 2);
-          nan_keys[tid] = 0;
-          __syncthreads();
-#pragma unroll
-          for (int x = 0; x < C::kPasses; ++x) {
-            const int row = 32 * warp + C::kRowsAtOnce * x + in_row;
-            if (((here >> x) & 1u) && byte_of(vbyte, x) == 255) atomicOr(nan_keys + row, 1u << blk);
-            if ((lost >> x) & 1u) atomicOr(nan_keys + row, 0x80000000u);  // a key that is not there
-          }
+          __syncwarp();
         }
-        write(sk, kcode, [&](int x) {
-          const int k = byte_of(kbyte, x);
-          if (plain) return (here >> x) & 1u ? scale_bits(k, 112) : 0u;
-          return !((here >> x) & 1u) ? 0u : k == 255 ? 0x7e00u : scale_bits(k, kbias);
-        });
-        fence_proxy_async_smem();
-        tc_fence_before();
-        __syncthreads();
-        if (tid == 0) {
-          tc_fence_after();
-#pragma unroll
-          for (int s = 0; s < D / 16; ++s) mma_bf16(tbase, desc_cols(uq, s), desc_cols(uk, s), kIdS, s > 0 ? 1u : 0u);
-          mma_commit(bar);
-        }
-        __syncwarp();
-        // under the product: V's operand, and the next tile's codes
-        find(key0 + kKeys);
-        load(kcode, kbyte, 0);
-        if (plain) {
-          write(sv, vcode, [&](int x) { return (vhere >> x) & 1u ? scale_bits(byte_of(vbyte, x), 112) : 0u; });
-          load(vcode, vbyte, 1);
-        }
-        wait(0, n_s++);
-
-        // ---- softmax of this thread's row, two passes over S
+        wait(kSFull, n_tile);
+        tc_fence_after();
+        const Tile& tile = tiles[n_tile & 1];
+        const bool plain = tile.plain;
         float f = factor;
-        if (!plain) f = fmaxf(f * pow2f(kbias - 112), 1.1754944e-38f);
-        const bool masked = key0 < inner_lo || key0 + kKeys > inner_hi;
-        const float cap = a.softcap * kLog2e, squeeze = a.softcap > 0.f ? 2.f * kLog2e / a.softcap : 0.f;
-        auto score = [&](uint32_t raw, int key) {
+        if (!plain) f = fmaxf(f * pow2f(tile.kbias - 112), 1.1754944e-38f);  // 0 would turn the mask's -inf into NaN
+        const bool masked = key0 < inner_lo || key0 + kKeys > inner_hi, simple = !masked && plain && !(a.softcap > 0.f);
+        const float cap = a.softcap * kLog2e, squeeze = a.softcap > 0.f ? f * 2.f * kLog2e / a.softcap : 0.f;
+        if (a.softcap > 0.f) f = 1.f;
+        auto score = [&](uint32_t raw, int j) {  // of key key0 + j, to be taken times f
           float v = __uint_as_float(raw);
-          if (a.softcap > 0.f) v = cap * (1.f - __fdividef(2.f, 1.f + ex2(v * f * squeeze)));  // tanh
-          if (masked) v = key >= lo && key < hi ? v : -INFINITY;
-          if (!plain && (nan_keys[key - key0] >> 31)) v = -INFINITY;
+          if (a.softcap > 0.f) v = cap * (1.f - __fdividef(2.f, 1.f + ex2(v * squeeze)));  // tanh x = 1 - 2 / (1 + e^2x)
+          if (masked) v = key0 + j >= lo && key0 + j < hi ? v : -INFINITY;
+          if (!plain && (tile.nan_keys[j] >> 31)) v = -INFINITY;
           return v;
         };
         float most = -INFINITY;
+        if (simple) {  // 64 columns in flight
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          tmem_ld32(ts + c * 32, r);
-          tmem_ld_wait();
-          if (!masked && plain && !(a.softcap > 0.f)) {
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[32], r2[32];
+            tmem_ld32(ts + c * 64, r);
+            tmem_ld32(ts + c * 64 + 32, r2);
+            tmem_ld_wait();
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[j & 3] = fmaxf(x[j & 3], __uint_as_float(r[j]));
+            for (int j = 0; j < 32; ++j) x[j & 3] = fmaxf(x[j & 3], fmaxf(__uint_as_float(r[j]), __uint_as_float(r2[j])));
             most = fmaxf(most, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) most = fmaxf(most, score(r[j], key0 + c * 32 + j));
           }
-        }
-        if (a.softcap > 0.f) f = 1.f;
-        const float next = fmaxf(m, most * f);
-        out_of_range = out_of_range || (next != -INFINITY && fabsf(next) > 65536.f);
-        if (n_tile > 0 && __any_sync(0xffffffffu, next != m)) {
-          const float keep = shrink(m, next);
-          l *= keep;
+        } else {
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = 0; c < 4; ++c) {
             uint32_t r[32];
-            tmem_ld32(to + c * 32, r);
+            tmem_ld32(ts + c * 32, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
-            tmem_st32(to + c * 32, r);
+            for (int j = 0; j < 32; ++j) most = fmaxf(most, score(r[j], c * 32 + j));
           }
-          tmem_st_wait();
+        }
+        most *= f;
+        // fp16 holds p up to 2^15.99: the maximum may lag behind by 0.9
+        const float next = most > m + 0.9f ? most : m;
+        out_of_range = out_of_range || (next != -INFINITY && fabsf(next) > 65536.f);
+        if (t > 0 && __any_sync(0xffffffffu, next != m)) {
+          const float keep = shrink(m, next);
+          l *= keep;
+          each_sum([&](uint32_t (&r)[32]) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+          });
         }
         m = next;
         const float d0 = m == -INFINITY ? 0.f : 15.f - m;  // p times 2^15
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
+          uint32_t r[32], h[16];
           tmem_ld32(ts + c * 32, r);
           tmem_ld_wait();
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t h[16];
-          if (!masked && plain && !(a.softcap > 0.f) && !out_of_range) {
+          if (simple && !__any_sync(0xffffffffu, out_of_range)) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float x = ex2(fmaf(__uint_as_float(r[2 * j]), f, d0)), y = ex2(fmaf(__uint_as_float(r[2 * j + 1]), f, d0));
@@ -351,144 +467,130 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           } else {
             // the product rounded before the maximum is taken off: a fused one would keep the bits
             // that rounding took from the maximum
-            f = a.softcap > 0.f ? factor * (plain ? 1.f : pow2f(kbias - 112)) : f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const float g = a.softcap > 0.f ? 1.f : f;
-              const float x = ex2(__fmul_rn(score(r[2 * j], key0 + c * 32 + 2 * j), g) + d0);
-              const float y = ex2(__fmul_rn(score(r[2 * j + 1], key0 + c * 32 + 2 * j + 1), g) + d0);
+              const float x = ex2(__fmul_rn(score(r[2 * j], c * 32 + 2 * j), f) + d0);
+              const float y = ex2(__fmul_rn(score(r[2 * j + 1], c * 32 + 2 * j + 1), f) + d0);
               sum[0] += x;
               sum[1] += y;
               h[j] = pack_half2(x, y);
             }
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4*>(piece_at(sp, tid, c * 32 + 8 * q)) = make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
+          tmem_st16(ts + c * 16, h);  // over columns of S that have been read
         }
+        tmem_st_wait();
 
-        // ---- P V: ordinarily one product, else one for each window of V's exponents, the largest first
-        int bias = vbias, most_byte = 254;
         bool dropped = false;  // this row's sums are too large for smaller units
-        while (true) {
+        const int windows = tile.windows;
+        for (int w = 0; w < windows && alive; ++w) {
           if (!plain) {
-            careful = true;
-            if (n_tile > 0) wait(1, n_o - 1);
+            if (w > 0) {
+              wait(kOFull, n_pv - 1);
+              tc_fence_after();
+            } else {
+              for (int j = 0; j < kKeys; ++j)
+                if (key0 + j >= lo && key0 + j < hi) poison |= tile.nan_keys[j] & 0xfu;
+            }
             // the row's sums to the unit of this window
-            const int want = bias - 112;
+            const int want = tile.bias[w] - 112;
+            const bool sums = t > 0 || w > 0;
             float big = 0.f;
-            if (n_tile > 0) {
-#pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t r[32];
-                tmem_ld32(to + c * 32, r);
-                tmem_ld_wait();
+            if (sums)
+              each_sum([&](uint32_t (&r)[32]) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) big = fmaxf(big, fabsf(__uint_as_float(r[j])));
-              }
-            }
+              });
             if (big == 0.f) unit = want;  // nothing to move
             const int top = static_cast<int>(__float_as_uint(big) >> 23) - 127;
             if (unit - want > min(126, max(0, 96 - top))) dropped = true;
             const int by = dropped ? 0 : unit - want;
             const float s0 = pow2f(max(by, -126)), s1 = pow2f(max(min(by + 126, 0), -126));
-            if (n_tile > 0 && __any_sync(0xffffffffu, by != 0)) {
-#pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t r[32];
-                tmem_ld32(to + c * 32, r);
-                tmem_ld_wait();
+            if (sums)
+              each_sum([&](uint32_t (&r)[32]) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * s0 * s1);
-                tmem_st32(to + c * 32, r);
+              });
+            unit -= by;
+            if (__any_sync(0xffffffffu, dropped)) {  // such a row's P becomes 0, the others' stay
+#pragma unroll 1
+              for (int c = 0; c < 2; ++c) {
+                uint32_t r[32];
+                tmem_ld32(ts + c * 32, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[j] = dropped ? 0u : r[j];
+                tmem_st32(ts + c * 32, r);
               }
               tmem_st_wait();
             }
-            unit -= by;
-            if (dropped) {
-#pragma unroll
-              for (int q = 0; q < 16; ++q) *reinterpret_cast<uint4*>(piece_at(sp, tid, 8 * q)) = make_uint4(0, 0, 0, 0);
-            }
-            write(sv, vcode, [&](int x) {
-              const int v = byte_of(vbyte, x);
-              return !((vhere >> x) & 1u) || v > most_byte ? 0u : scale_bits(v, bias);
-            });
           }
-          fence_proxy_async_smem();
           tc_fence_before();
-          __syncthreads();
-          if (tid == 0) {
-            tc_fence_after();
+          arrive(kPFull);
+          if (warp == 0) {
+            wait(kVFull, n_pv);
+            wait(kPFull, n_pv);
+            if (alive && elect_one()) {
+              tc_fence_after();
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
-              mma_bf16(tbase + 128, desc_cols(up_, s), desc_rows(uv, s), kIdO, (n_tile > 0 || s > 0) ? 1u : 0u);
-            mma_commit(bar + 1);
+              for (int s = 0; s < kKeys / 16; ++s)
+                mma_f16_ts(tbase + 128, tbase + 8 * s, dv + step_rows(s), kIdO, t > 0 || w > 0 || s > 0 ? 1u : 0u);
+              mma_commit(bar + kOFull);
+            }
+            __syncwarp();
           }
-          __syncwarp();
-          ++n_o;
-          ++n_tile;
-          if (plain) break;
-          int below = 0;  // the largest byte that no window has held yet
-#pragma unroll
-          for (int x = 0; x < C::kPasses; ++x) {
-            const int v = byte_of(vbyte, x);
-            if (((vhere >> x) & 1u) && v <= bias && v > 1) below = max(below, v);
-          }
-          below = block_max(below);
-          if (below == 0) break;
-          most_byte = bias;
-          bias = below - 28;
+          ++n_pv;
         }
-        if (!plain) {
-          for (int j = 0; j < kKeys; ++j)
-            if (key0 + j >= lo && key0 + j < hi) poison |= nan_keys[j] & 0xfu;
-          load(vcode, vbyte, 1);
-        }
+        ++n_tile;
       }
 
       // ---- the result, or a part of it
-      if (n_tile > 0) wait(1, n_o - 1);
-      const bool whole = list.whole();
-      const float keep = (l == 0.f ? 0.f : 1.f / l) * (whole && a.sink != nullptr ? share_beside(a.sink[head * G + (row0 + min(tid, rows - 1)) % G], m, l) : 1.f);
-      const float power = pow2f(max(-126, min(126, unit)));
-      const int i = row0 + tid;
-      const int64_t row = (static_cast<int64_t>(b) * a.H + head * G + i % G) * a.T + i / G;
-      const int64_t slot = list.part_row() + tid;
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        if (n_tile > 0) {
-          tmem_ld32(to + c * 32, r);
-          tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = 0;
+      if (take > 0) {
+        if (count > 0) {
+          wait(kOFull, n_pv - 1);
+          tc_fence_after();
         }
-        if (tid >= rows) continue;
-        const float add = (poison >> c) & 1u ? NAN : 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float o[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(r[8 * q + j]) * keep * power + add;
-          if (whole) {
-            Few<T, 8> y;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y.v[j] = static_cast<T>(o[j]);
-            *reinterpret_cast<Few<T, 8>*>(static_cast<T*>(a.out) + row * D + c * 32 + 8 * q) = y;
+        const bool whole = list.whole();
+        const int i = row0 + row, h = head * G + min(i, G * a.T - 1) % G;
+        const float keep = (l == 0.f ? 0.f : 1.f / l) * (whole && a.sink != nullptr ? share_beside(a.sink[h], m, l) : 1.f);
+        const float power = pow2f(max(-126, min(126, unit)));
+        const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.T + i / G, slot = list.part_row() + row;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          if (count > 0) {
+            tmem_ld32(to + c * 32, r);
+            tmem_ld_wait();
           } else {
-            float4* to_part = reinterpret_cast<float4*>(a.part_out + slot * D + c * 32 + 8 * q);
-            to_part[0] = make_float4(o[0], o[1], o[2], o[3]);
-            to_part[1] = make_float4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = 0;
+          }
+          if (row >= rows) continue;
+          const float add = (poison >> c) & 1u ? NAN : 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float o[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(r[8 * q + j]) * keep * power + add;
+            if (whole) {
+              Few<T, 8> y;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) y.v[j] = static_cast<T>(o[j]);
+              *reinterpret_cast<Few<T, 8>*>(static_cast<T*>(a.out) + at * D + c * 32 + 8 * q) = y;
+            } else {
+              float4* out = reinterpret_cast<float4*>(a.part_out + slot * D + c * 32 + 8 * q);
+              out[0] = make_float4(o[0], o[1], o[2], o[3]);
+              out[1] = make_float4(o[4], o[5], o[6], o[7]);
+            }
           }
         }
+        if (!whole && row < rows) a.part_ml[slot] = make_float2(m, l);
       }
-      if (!whole && tid < rows) a.part_ml[slot] = make_float2(m, l);
       tc_fence_before();  // the next segment's products overwrite the sums
     }
-    if (!alive || !list.next(a, row_tiles)) break;
-    __syncthreads();
+    if (count > 0) ++n_seg;
+    if (!__syncthreads_and(alive)) break;
+    if (!list.next(a, row_tiles)) break;
   }
   tc_fence_before();
   __syncthreads();

@@ -365,7 +365,7 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   a.softcap = static_cast<float>(softcap);
   a.err = err.data_ptr<int>();
   TORCH_CHECK(B <= 65535 && H * T <= (1 << 26), "fp4_kv_attention: at most 65535 sequences and 2^26 query rows in each");
-  const bool many = d >= 64 && H / Hk * T >= kTileRows;
+  const bool many = d >= 64 && H / Hk * T >= kTileRows && pages.size(0) > 0;
   const Fp4AttnPlan plan = many ? fp4_attn_tile_plan(a) : fp4_attn_rows_plan(a, static_cast<int>(d));
   TORCH_CHECK(plan.units < INT32_MAX, "fp4_kv_attention: more than 2^31 tiles of work in one call");
   a.blocks = plan.blocks;
