@@ -403,12 +403,11 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         const bool plain = tile.plain;
         float f = factor;
         if (!plain) f = fmaxf(f * pow2f(tile.kbias - 112), 1.1754944e-38f);  // 0 would turn the mask's -inf into NaN
-        const bool masked = key0 < inner_lo || key0 + kKeys > inner_hi, simple = !masked && plain && !(a.softcap > 0.f);
+        const bool masked = key0 < inner_lo || key0 + kKeys > inner_hi, simple = !masked && plain;
         const float cap = a.softcap * kLog2e, squeeze = a.softcap > 0.f ? f * 2.f * kLog2e / a.softcap : 0.f;
-        if (a.softcap > 0.f) f = 1.f;
-        auto score = [&](uint32_t raw, int j) {  // of key key0 + j, to be taken times f
+        auto capped = [&](float v) { return cap * (1.f - __fdividef(2.f, 1.f + ex2(v * squeeze))); };  // tanh x = 1 - 2 / (1 + e^2x)
+        auto visible = [&](uint32_t raw, int j) {  // the raw score of key key0 + j, or -inf
           float v = __uint_as_float(raw);
-          if (a.softcap > 0.f) v = cap * (1.f - __fdividef(2.f, 1.f + ex2(v * squeeze)));  // tanh x = 1 - 2 / (1 + e^2x)
           if (masked) v = key0 + j >= lo && key0 + j < hi ? v : -INFINITY;
           if (!plain && (tile.nan_keys[j] >> 31)) v = -INFINITY;
           return v;
@@ -433,10 +432,11 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
             tmem_ld32(ts + c * 32, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) most = fmaxf(most, score(r[j], c * 32 + j));
+            for (int j = 0; j < 32; ++j) most = fmaxf(most, visible(r[j], c * 32 + j));
           }
         }
-        most *= f;
+        if (a.softcap > 0.f) most = most == -INFINITY ? most : capped(most);  // tanh keeps the order
+        else most *= f;
         // fp16 holds p up to 2^15.99: the maximum may lag behind by 0.9
         const float next = most > m + 0.9f ? most : m;
         out_of_range = out_of_range || (next != -INFINITY && fabsf(next) > 65536.f);
@@ -456,25 +456,27 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           tmem_ld32(ts + c * 32, r);
           tmem_ld_wait();
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          if (simple && !__any_sync(0xffffffffu, out_of_range)) {
+          auto weigh = [&](auto&& exponent) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const float x = ex2(fmaf(__uint_as_float(r[2 * j]), f, d0)), y = ex2(fmaf(__uint_as_float(r[2 * j + 1]), f, d0));
+              const float x = ex2(exponent(2 * j)), y = ex2(exponent(2 * j + 1));
               sum[(2 * j) & 3] += x;
               sum[(2 * j + 1) & 3] += y;
               h[j] = pack_half2(x, y);
             }
+          };
+          if (a.softcap > 0.f) {
+            if (simple) weigh([&](int j) { return capped(__uint_as_float(r[j])) + d0; });
+            else weigh([&](int j) {
+              const float v = visible(r[j], c * 32 + j);
+              return v == -INFINITY ? v : capped(v) + d0;
+            });
+          } else if (simple && !__any_sync(0xffffffffu, out_of_range)) {
+            weigh([&](int j) { return fmaf(__uint_as_float(r[j]), f, d0); });
           } else {
             // the product rounded before the maximum is taken off: a fused one would keep the bits
             // that rounding took from the maximum
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float x = ex2(__fmul_rn(score(r[2 * j], c * 32 + 2 * j), f) + d0);
-              const float y = ex2(__fmul_rn(score(r[2 * j + 1], c * 32 + 2 * j + 1), f) + d0);
-              sum[0] += x;
-              sum[1] += y;
-              h[j] = pack_half2(x, y);
-            }
+            weigh([&](int j) { return __fmul_rn(visible(r[j], c * 32 + j), f) + d0; });
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_st16(ts + c * 16, h);  // over columns of S that have been read

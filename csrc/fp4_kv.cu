@@ -231,7 +231,15 @@ torch::Tensor rows_aligned(const torch::Tensor& t) {
   return ok ? t : t.contiguous();
 }
 
-constexpr int kTileRows = 64;
+// Which of the two attention kernels.  One time grows with 16-row tiles times 32-key steps (about 2 ns
+// each at d = 128, behind 10 us), the other with 128-row tiles times 128 keys (20 ns behind 20 us):
+// 64 sequences of 4096 keys and 16 heads take 47 and 54 us with 3 tokens each (28k steps), 58 and 55
+// with 4 (37k), 78 and 58 with 6 (55k); 8 sequences of 8192 keys 43 and 48 us with 16 tokens (33k).
+constexpr int64_t kManySteps = 36000;
+
+bool many_rows(int64_t groups, int64_t rows, int64_t keys) {
+  return rows > 32 && groups * ((rows + 15) / 16) * ((keys + 31) / 32) >= kManySteps;
+}
 
 RowsArgs rows_args(const torch::Tensor& pages, const torch::Tensor& slots, int64_t d, const char* who) {
   RowsArgs a{};
@@ -365,7 +373,8 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   a.softcap = static_cast<float>(softcap);
   a.err = err.data_ptr<int>();
   TORCH_CHECK(B <= 65535 && H * T <= (1 << 26), "fp4_kv_attention: at most 65535 sequences and 2^26 query rows in each");
-  const bool many = d >= 64 && H / Hk * T >= kTileRows && pages.size(0) > 0;
+  const int64_t keys = window > 0 ? std::min<int64_t>(table.size(1) * a.R, window + T) : table.size(1) * a.R;
+  const bool many = d >= 64 && pages.size(0) > 0 && many_rows(B * Hk, H / Hk * T, keys);
   const Fp4AttnPlan plan = many ? fp4_attn_tile_plan(a) : fp4_attn_rows_plan(a, static_cast<int>(d));
   TORCH_CHECK(plan.units < INT32_MAX, "fp4_kv_attention: more than 2^31 tiles of work in one call");
   a.blocks = plan.blocks;

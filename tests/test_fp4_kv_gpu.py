@@ -9,13 +9,19 @@ from tests import _fp4_oracle as oracle
 pytestmark = pytest.mark.gpu
 
 
+def _with_room(table, room, rows):
+    """Tables wide enough for ``room`` keys: with many query rows the tensor-core tiles run by then."""
+    return torch.nn.functional.pad(table, (0, max(0, -(-room // rows) - table.shape[1])), value=-1)
+
+
 def _attend_case(cuda, lens, *, h, hk, d, rows, t=1, window=0, sink=None, softcap=None, dtype=torch.bfloat16,
-                 qscale=1.0, spread=None, seed=0, one_hot=False):
+                 qscale=1.0, spread=None, seed=0, one_hot=False, room=0):
     from saint_llm_b200.ops.fp4_kv import fp4_kv_attention
     from saint_llm_b200.ops.gemm import check_errors
 
     gen = torch.Generator().manual_seed(seed)
     pages, table, lengths = oracle.filled(lens, hk=hk, d=d, rows=rows, gen=gen, device=cuda, spread=spread)
+    table = _with_room(table, room, rows)
     q = (qscale * torch.randn(len(lens), h, t, d, generator=gen)).to(cuda, dtype)
     sl = None if sink is None else sink.to(cuda) if torch.is_tensor(sink) else torch.randn(h, generator=gen).to(cuda)
     got = fp4_kv_attention(q, pages, table, lengths, window=window, sink=sl, softcap=softcap)
@@ -81,25 +87,28 @@ def test_attention_long_cache_in_splits(cuda):
     _attend_case(cuda, [9001], h=4, hk=4, d=64, rows=128, dtype=torch.float16)
 
 
+@pytest.mark.parametrize("room", [0, 1 << 20])
 @pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
-def test_attention_of_many_rows(cuda, d, dtype):
-    """64 query rows per K / V head and more: the tensor-core tiles, at their edges."""
-    _attend_case(cuda, [128, 129, 300, 0, 39, 1], h=4, hk=2, d=d, rows=16, t=40, dtype=dtype, sink=True)
-    _attend_case(cuda, [700, 256], h=3, hk=1, d=d, rows=48, t=70, dtype=dtype, softcap=12.0, qscale=3.0)
-    _attend_case(cuda, [513, 140], h=16, hk=1, d=d, rows=64, t=9, dtype=dtype, window=100, sink=True)
-    _attend_case(cuda, [3000], h=64, hk=1, d=d, rows=128, t=2, dtype=dtype)
+def test_attention_of_many_rows(cuda, d, dtype, room):
+    """Both kernels at the edges of their tiles: 16 rows by 32 keys, and in wide tables 128 by 128."""
+    _attend_case(cuda, [128, 129, 300, 0, 39, 1], h=4, hk=2, d=d, rows=16, t=40, dtype=dtype, sink=True, room=room)
+    _attend_case(cuda, [700, 256], h=3, hk=1, d=d, rows=48, t=70, dtype=dtype, softcap=12.0, qscale=3.0, room=room)
+    _attend_case(cuda, [513, 140], h=16, hk=1, d=d, rows=64, t=9, dtype=dtype, window=100, sink=True,
+                 room=room)
+    _attend_case(cuda, [3000], h=64, hk=1, d=d, rows=128, t=2, dtype=dtype, room=room)
+    _attend_case(cuda, [90, 64, 10], h=4, hk=2, d=d, rows=32, t=20, dtype=dtype, window=30, softcap=9.0, room=room)
 
 
 @pytest.mark.parametrize("spread", [6, 30, 55])
 def test_attention_of_many_rows_of_very_different_size(cuda, spread):
-    _attend_case(cuda, [5, 64, 333], h=8, hk=1, d=128, rows=32, t=16, spread=spread, qscale=8.0)
-    _attend_case(cuda, [260], h=8, hk=2, d=64, rows=16, t=33, spread=spread, qscale=30.0)
+    _attend_case(cuda, [5, 64, 333], h=8, hk=1, d=128, rows=32, t=16, spread=spread, qscale=8.0, room=1 << 20)
+    _attend_case(cuda, [260], h=8, hk=2, d=64, rows=16, t=33, spread=spread, qscale=30.0, room=1 << 20)
 
 
 def test_attention_of_many_rows_sharp_scores(cuda):
-    _attend_case(cuda, [300, 200], h=8, hk=1, d=128, rows=64, t=20, qscale=60.0)
-    _attend_case(cuda, [300], h=8, hk=1, d=64, rows=64, t=20, qscale=0.0)
-    _attend_case(cuda, [300], h=8, hk=1, d=128, rows=64, t=20, qscale=2.0 ** 60, one_hot=True)
+    _attend_case(cuda, [300, 200], h=8, hk=1, d=128, rows=64, t=20, qscale=60.0, room=1 << 20)
+    _attend_case(cuda, [300], h=8, hk=1, d=64, rows=64, t=20, qscale=0.0, room=1 << 20)
+    _attend_case(cuda, [300], h=8, hk=1, d=128, rows=64, t=20, qscale=2.0 ** 60, one_hot=True, room=1 << 20)
 
 
 def test_attention_of_many_rows_nan_and_bad_pages(cuda):
@@ -108,6 +117,7 @@ def test_attention_of_many_rows_nan_and_bad_pages(cuda):
 
     gen = torch.Generator().manual_seed(11)
     pages, table, lengths = oracle.filled([200, 180], hk=1, d=128, rows=16, gen=gen, device=cuda)
+    table = _with_room(table, 1 << 20, 16)
     q = torch.randn(2, 8, 30, 128, generator=gen).to(cuda, torch.bfloat16)
     clean = fp4_kv_attention(q, pages, table, lengths)
     for which in range(2):
