@@ -49,6 +49,8 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
                                int64_t window, c10::optional<torch::Tensor> sink, double softcap, double scale,
                                torch::Tensor err);
 // pages.cu
+torch::Tensor reserve_rows(torch::Tensor table, torch::Tensor lengths, torch::Tensor refcount, torch::Tensor rows,
+                           int64_t count, int64_t page_rows, torch::Tensor err);
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> fork_pages(torch::Tensor pool, torch::Tensor table,
                                                                    torch::Tensor lengths, torch::Tensor refcount,
                                                                    torch::Tensor parents, torch::Tensor children,
@@ -206,6 +208,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp4_kv_write", &sv4::fp4_kv_write);
   m.def("fp4_kv_read", &sv4::fp4_kv_read);
   m.def("fp4_kv_attention", &sv4::fp4_kv_attention);
+  m.def("reserve_rows", &sv4::reserve_rows);
   m.def("fork_pages", &sv4::fork_pages);
   m.def("compact_pages", &sv4::compact_pages);
   m.def("decode_attention", &sv4::decode_attention);

@@ -64,6 +64,83 @@ __device__ __forceinline__ void copy_piece(uint8_t* to, const uint8_t* from, int
     if (static_cast<int>(threadIdx.x) + x * kCopyThreads < n) dst[threadIdx.x + x * kCopyThreads] = v[x];
 }
 
+// The first `need` free pages in ascending order, by the planning block; returns how many were found.
+__device__ __forceinline__ int find_free(const int* refcount, int n_pages, int need, int* found) {
+  int have = 0;
+  for (int p0 = 0; p0 < n_pages && have < need; p0 += kPlan) {
+    const int p = p0 + threadIdx.x;
+    int total;
+    const int is_free = p < n_pages && refcount[p] == 0;
+    const int rank = have + block_scan(is_free, &total);
+    if (is_free && rank < need) found[rank] = p;
+    have += total;
+  }
+  __syncthreads();
+  return min(have, need);
+}
+
+struct ReserveArgs {
+  int* table;
+  int* lengths;
+  int* refcount;
+  const int* rows;
+  int64_t* slots;  // (n, count)
+  int* found;      // (n * pages that `count` rows can open)
+  int S, P, n, n_pages, R, count;
+  int* err;
+};
+
+// One block: the pages that `count` more rows of each sequence open, in the order of the sequences;
+// all or nothing.  The pages' ids go into the table, the rows' slots out.
+__global__ void __launch_bounds__(kPlan) reserve_rows_kernel(const ReserveArgs a) {
+  // pages that sequence i needs, with its row and length; -1: out of range
+  auto needs = [&](int i, int& row, int& len, int* err) {
+    row = a.rows[i];
+    len = 0;
+    if (!index_ok(row, 0, a.S, err)) return -1;
+    len = a.lengths[row];
+    if (!index_ok(len, 0, static_cast<int64_t>(a.P) * a.R - a.count + 1, err)) return -1;
+    return (len + a.count + a.R - 1) / a.R - (len + a.R - 1) / a.R;
+  };
+  int need = 0, bad = 0;
+  for (int i0 = 0; i0 < a.n; i0 += kPlan) {
+    const int i = i0 + threadIdx.x;
+    int row, len, total;
+    const int pages = i < a.n ? needs(i, row, len, a.err) : 0;
+    bad += __syncthreads_count(pages < 0);
+    block_scan(max(pages, 0), &total);
+    need += total;
+  }
+  const bool fits = bad == 0 && find_free(a.refcount, a.n_pages, need, a.found) == need;
+  if (bad == 0 && !fits) record_error(a.err, kErrPages);
+  int before = 0;
+  for (int i0 = 0; i0 < a.n && fits; i0 += kPlan) {
+    const int i = i0 + threadIdx.x;
+    int row = 0, len = 0, total;
+    const int pages = i < a.n ? needs(i, row, len, nullptr) : 0;
+    const int first = before + block_scan(pages, &total);
+    for (int x = 0; x < pages; ++x) {
+      const int page = a.found[first + x];
+      a.table[static_cast<int64_t>(row) * a.P + (len + a.R - 1) / a.R + x] = page;
+      a.refcount[page] = 1;
+    }
+    before += total;
+  }
+  __syncthreads();
+  for (int64_t x = threadIdx.x; x < static_cast<int64_t>(a.n) * a.count; x += kPlan) {
+    int64_t slot = -1;
+    if (fits) {
+      const int row = a.rows[x / a.count];
+      const int pos = a.lengths[row] + static_cast<int>(x % a.count);
+      slot = static_cast<int64_t>(a.table[static_cast<int64_t>(row) * a.P + pos / a.R]) * a.R + pos % a.R;
+    }
+    a.slots[x] = slot;
+  }
+  __syncthreads();
+  if (fits)
+    for (int i = threadIdx.x; i < a.n; i += kPlan) a.lengths[a.rows[i]] += a.count;
+}
+
 struct ForkArgs {
   uint8_t* pool;
   int64_t page_bytes;
@@ -114,19 +191,8 @@ __global__ void __launch_bounds__(kPlan) fork_plan_kernel(const ForkArgs a) {
     if (i < a.F) a.fresh[i] = copies ? rank : -1;  // the rank now, the page below
     need += total;
   }
-  // the first `need` free pages go into the tail of `fresh`
-  int* found = a.fresh + a.F + 1;
-  int have = 0;
-  for (int p0 = 0; p0 < a.n_pages && have < need; p0 += kPlan) {
-    const int p = p0 + threadIdx.x;
-    int total;
-    const int is_free = p < a.n_pages && a.refcount[p] == 0;
-    const int rank = have + block_scan(is_free, &total);
-    if (is_free && rank < need) found[rank] = p;
-    have += total;
-  }
-  __syncthreads();
-  const bool fits = have >= need;
+  int* found = a.fresh + a.F + 1;  // the tail of `fresh`
+  const bool fits = find_free(a.refcount, a.n_pages, need, found) == need;
   if (!fits) record_error(a.err, kErrPages);
   for (int i = threadIdx.x; i < a.F; i += kPlan) {
     const int rank = a.fresh[i];
@@ -287,6 +353,41 @@ int64_t check_pool(const torch::Tensor& pool, const torch::Tensor& table, const 
 }
 
 }  // namespace
+
+// In place: `count` more rows for each of `rows`; returns their slots (n, count).
+torch::Tensor reserve_rows(torch::Tensor table, torch::Tensor lengths, torch::Tensor refcount, torch::Tensor rows,
+                           int64_t count, int64_t page_rows, torch::Tensor err) {
+  TORCH_CHECK(table.is_cuda() && table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous(),
+              "reserve_rows: table must be a contiguous CUDA (rows, pages) int32 tensor");
+  auto vec = [&](const torch::Tensor& t) {
+    return t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.device() == table.device();
+  };
+  TORCH_CHECK(vec(lengths) && lengths.size(0) == table.size(0) && vec(refcount) && vec(rows),
+              "reserve_rows: lengths, refcount and rows must be contiguous int32 vectors on the table's device");
+  TORCH_CHECK(count > 0 && page_rows > 0 && table.size(1) * page_rows <= INT32_MAX && count <= INT32_MAX / 2,
+              "reserve_rows: count and page_rows must be positive");
+  c10::cuda::CUDAGuard guard(table.device());
+  auto slots = at::detail::empty_cuda({rows.size(0), count}, at::kLong, table.device(), std::nullopt);
+  if (rows.size(0) == 0) return slots;
+  auto found = ints({rows.size(0) * ((count + page_rows - 1) / page_rows)}, table);
+  ReserveArgs a{};
+  a.table = table.data_ptr<int>();
+  a.lengths = lengths.data_ptr<int>();
+  a.refcount = refcount.data_ptr<int>();
+  a.rows = rows.data_ptr<int>();
+  a.slots = slots.data_ptr<int64_t>();
+  a.found = found.data_ptr<int>();
+  a.S = static_cast<int>(table.size(0));
+  a.P = static_cast<int>(table.size(1));
+  a.n = static_cast<int>(rows.size(0));
+  a.n_pages = static_cast<int>(refcount.size(0));
+  a.R = static_cast<int>(page_rows);
+  a.count = static_cast<int>(count);
+  a.err = err.data_ptr<int>();
+  reserve_rows_kernel<<<1, kPlan, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return slots;
+}
 
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> fork_pages(torch::Tensor pool, torch::Tensor table,
                                                                    torch::Tensor lengths, torch::Tensor refcount,

@@ -1,10 +1,11 @@
-"""Page operators of a paged cache: fork, free and compact, on the device.
+"""Page operators of a paged cache: reserve, fork, free and compact, on the device.
 
 The state of a pool is ``table`` (S, P) int32 (row s: the page ids of sequence s in order, -1
 behind the last), ``lengths`` (S,) int32 rows per sequence and ``refcount`` (n_pages,) int32: how
 many table rows hold a page, 0 meaning free.  ``pool`` is any contiguous tensor (n_pages, ...):
-bf16 rows, 4-bit pages of many layers; its bytes are only moved.  The functions return new state
-tensors and change ``pool`` in place; nothing is read on the host.
+bf16 rows, 4-bit pages of many layers; its bytes are only moved.  ``fork_pages`` and
+``compact_pages`` return new state tensors and change ``pool`` in place, ``reserve_rows`` changes
+the state in place (a captured decode step calls it); nothing is read on the host.
 
 CPU tensors (and ``backend.eager_mode()``) take the definitions below; CUDA tensors run
 ``csrc/pages.cu``, where an index out of range or a pool with too few free pages is recorded and
@@ -28,6 +29,42 @@ def _check(pool: Tensor, table: Tensor, refcount: Tensor) -> None:
         raise ValueError("table must be (rows, pages) int32 and refcount one int32 per page")
     if table.device != pool.device or refcount.device != pool.device:
         raise ValueError(f"pool, table and refcount must be on one device, got {pool.device} and {table.device}")
+
+
+def reserve_rows(table: Tensor, lengths: Tensor, refcount: Tensor, rows: Tensor, count: int, *,
+                 page_rows: int) -> Tensor:
+    """Room for ``count`` more rows of each of the sequences ``rows`` (n,) int32, in place: pages are
+    taken (the lowest free ones, in the order of ``rows``) where a row opens one, the lengths grow.
+    Returns the rows' slots (n, count) int64 = page * page_rows + row.  ``rows`` must differ from one
+    another.  With too few free pages, or a table too narrow, nothing changes, every slot is -1 (which
+    writes skip) and an error is raised (on CUDA: by ``check_errors``)."""
+    if backend.native_for(table):
+        return backend.ext().reserve_rows(table, lengths, refcount, rows, count, page_rows, error_word(table.device))
+    from saint_llm_b200.infer.paged_kv import PoolExhausted
+
+    if table.dim() != 2 or rows.dim() != 1 or lengths.shape != table.shape[:1] or count <= 0 or page_rows <= 0:
+        raise ValueError("table must be (rows, pages), lengths one per table row; count and page_rows positive")
+    free = (refcount == 0).nonzero().flatten().tolist()
+    taken = 0
+    new: list[tuple[int, int, int]] = []
+    for r in rows.tolist():
+        if not 0 <= r < table.shape[0]:
+            raise IndexError(f"row {r} of {table.shape[0]}")
+        n = int(lengths[r])
+        if n + count > table.shape[1] * page_rows:
+            raise IndexError(f"{n + count} rows in a table for {table.shape[1] * page_rows}")
+        for c in range(-(-n // page_rows), -(-(n + count) // page_rows)):
+            if taken == len(free):
+                raise PoolExhausted(f"{len(free)} of {len(refcount)} pages free, more needed")
+            new.append((r, c, free[taken]))
+            taken += 1
+    for r, c, p in new:
+        table[r, c] = p
+        refcount[p] = 1
+    pos = lengths[rows.long()].long().unsqueeze(1) + torch.arange(count, device=table.device)
+    slots = table[rows.long()].long().gather(1, pos // page_rows) * page_rows + pos % page_rows
+    lengths[rows.long()] += count
+    return slots
 
 
 def fork_pages(pool: Tensor, table: Tensor, lengths: Tensor, refcount: Tensor, parents: Tensor, children: Tensor, *,
@@ -104,4 +141,4 @@ def compact_pages(pool: Tensor, table: Tensor, refcount: Tensor) -> tuple[Tensor
     return torch.where(ids >= 0, where[ids.clamp(min=0)].int(), -1).int(), refs, n.int()
 
 
-__all__ = ["compact_pages", "fork_pages"]
+__all__ = ["compact_pages", "fork_pages", "reserve_rows"]
