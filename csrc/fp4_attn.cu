@@ -135,12 +135,23 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
       const int head = y / tiles_per_head, row0 = (y % tiles_per_head) * C::kRows;
       const int rows = min(C::kRows, G * a.T - row0);
       // one past the last key that row i (token t) may see; rows behind the last repeat it
-      auto end_of = [&](int i) { return sp.len - a.T + (row0 + min(i, rows - 1)) / G + 1; };
+      auto end_of = [&](int i) { return a.T == 1 ? sp.len : sp.len - a.T + (row0 + min(i, rows - 1)) / G + 1; };
       const int last = end_of(C::kRows - 1), inner_hi = end_of(0);
       const int first = a.window > 0 ? max(0, inner_hi - a.window) : 0, inner_lo = a.window > 0 ? max(0, last - a.window) : 0;
       const int mine = take > warp ? (take - warp + kWarps - 1) / kWarps : 0;
       const int base = sp.start + (from_tile + warp) * kTile;  // the warp's first key
       const int* table = a.table + static_cast<int64_t>(b) * a.P;
+
+      // this thread's part of the queries, on its way while the first tiles are found: rows 8 z + g, dims
+      // c d/4 .. (c + 1) d/4
+      uint4 raw[NT][C::kC];
+#pragma unroll
+      for (int z = 0; z < NT; ++z) {
+        const int i = row0 + min(8 * z + g, rows - 1), t = a.T == 1 ? 0 : i / G;
+        const T* row = static_cast<const T*>(a.q) + b * a.q_b + (head * G + i - t * G) * a.q_h + t * a.q_t;
+#pragma unroll
+        for (int k = 0; k < C::kC; ++k) raw[z][k] = *reinterpret_cast<const uint4*>(row + c * (D / 4) + 8 * k);
+      }
 
       // Where the halves (16 keys) of sixteen coming tiles lie: lane 2 i + h holds half h of tile i.
       auto look_up = [&](int batch, const uint8_t*& slab, int& in_page) {
@@ -157,10 +168,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           }
         }
       };
-      const uint8_t *slab_now, *slab_next;
-      int in_now, in_next;
-      look_up(0, slab_now, in_now);
-      look_up(1, slab_next, in_next);
+      const uint8_t *slab_now, *slab_next = nullptr;
+      int in_now, in_next = 0;
       uint32_t present = 0;  // two bits per stage: its halves that were copied
       int fill = 0, stage = 0;  // the next stages to copy into and to compute
 
@@ -203,26 +212,24 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
         present = (present & ~(3u << (2 * fill))) | (((s0 != nullptr ? 1u : 0u) | (s1 != nullptr ? 2u : 0u)) << (2 * fill));
         fill = fill + 1 == C::kStages ? 0 : fill + 1;
       };
+      look_up(0, slab_now, in_now);
 #pragma unroll
       for (int i = 0; i < C::kStages - 1; ++i) {
         issue(i);
         copy_commit();
       }
+      if (mine > 16) look_up(1, slab_next, in_next);
 
-      // ---- q as the B operand: row 8 z + g, dims c d/4 .. (c + 1) d/4, scaled to fp16's top
+      // ---- q as the B operand, scaled to fp16's top
       uint32_t qf[NT][C::kC][4];
       float factor[NT][2];  // raw score -> softmax units, rows 8 z + 2 c + x
       int hi[NT][2];        // one past the last visible key, for the same rows
 #pragma unroll
       for (int z = 0; z < NT; ++z) {
-        const int i = row0 + min(8 * z + g, rows - 1);
-        const T* row = static_cast<const T*>(a.q) + b * a.q_b + (head * G + i % G) * a.q_h + (i / G) * a.q_t;
-        uint4 raw[C::kC];
         float amax = 0.f;
 #pragma unroll
         for (int k = 0; k < C::kC; ++k) {
-          raw[k] = *reinterpret_cast<const uint4*>(row + c * (D / 4) + 8 * k);
-          const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+          const uint32_t w[4] = {raw[z][k].x, raw[z][k].y, raw[z][k].z, raw[z][k].w};
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const float2 f = two_floats(w[x], T{});
@@ -237,7 +244,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
         const float unit = pow2f(max(-up, -126)) * nat;
 #pragma unroll
         for (int k = 0; k < C::kC; ++k) {
-          const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+          const uint32_t w[4] = {raw[z][k].x, raw[z][k].y, raw[z][k].z, raw[z][k].w};
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
             const float2 v = two_floats(w[p], T{});
@@ -619,7 +626,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           for (int n = 0; n < 2; ++n) {
             const int i = 8 * z + 2 * c + n;
             if (i >= rows) continue;
-            const int h = head * G + (row0 + i) % G, t = (row0 + i) / G;
+            const int t = a.T == 1 ? 0 : (row0 + i) / G, h = head * G + row0 + i - t * G;
             const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.T + t;
             const float keep = whole && a.sink != nullptr ? share_beside(a.sink[h], top[z][n], whole_l[z][n]) : 1.f;
             Few<float, 2 * kX> o;

@@ -103,20 +103,25 @@ struct Work {
   }
   __device__ static int units_of(const Span& s) { return s.tiles > 0 ? s.tiles + Cost : 0; }
 
-  // Sum of a segment's units for b < upto and over all b, by the whole block (every thread gets both).
+  // Sum of a segment's units for b < upto and over all b (every thread gets both).  Each warp counts for
+  // itself while that takes few loads, else the block's warps share them and meet.
   __device__ static void count_units(const Fp4AttnArgs& a, int upto, int& before, int& all) {
     __shared__ int part[2][32];
+    const bool alone = a.B <= 256;
+    const int step = alone ? 32 : blockDim.x;
     int mine = 0, below = 0;
-    for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
+#pragma unroll 2
+    for (int b = alone ? threadIdx.x & 31 : threadIdx.x; b < a.B; b += step) {
       const int n = units_of(span_of(a, b));
       mine += n;
       if (b < upto) below += n;
     }
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    below = __reduce_add_sync(0xffffffffu, below);
+    all = __reduce_add_sync(0xffffffffu, mine);
+    before = __reduce_add_sync(0xffffffffu, below);
+    if (alone) return;
     if ((threadIdx.x & 31) == 0) {
-      part[0][threadIdx.x >> 5] = below;
-      part[1][threadIdx.x >> 5] = mine;
+      part[0][threadIdx.x >> 5] = before;
+      part[1][threadIdx.x >> 5] = all;
     }
     __syncthreads();
     before = all = 0;
