@@ -19,7 +19,8 @@
 //   unit by powers of two.
 // * q is scaled by a power of two per row to the top of fp16's range (bf16 keeps its 8 bits, what
 //   falls below 2^-38 of the row's largest is lost).  p is held times 2^15: fp16's 11 bits for
-//   weights down to 2^-29 of the largest.
+//   weights down to 2^-29 of the largest.  A row's maximum is left as it is while the new one is at
+//   most 0.9 larger (log2), for which fp16 has room: the sums are rescaled less often.
 // * Operand order: dims and keys may be summed in any order, so a thread's operands are chosen to
 //   lie together: d/4 dims of a key for K; for V the d/16 bytes of its d/8 output dims, two keys'
 //   nibbles merged into the bytes that cvt turns into a pair.
@@ -454,7 +455,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
             float x = fmaxf(fmaxf(s[0][z][n], s[0][z][2 + n]), fmaxf(s[1][z][n], s[1][z][2 + n]));
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-            next[z][n] = fmaxf(m[z][n], x * f[z][n]);
+            // fp16 holds p up to 2^15.99: the maximum may lag behind by 0.9
+            next[z][n] = x * f[z][n] > m[z][n] + 0.9f ? x * f[z][n] : m[z][n];
             moved = moved || next[z][n] != m[z][n];
             most = fmaxf(most, next[z][n] == -INFINITY ? 0.f : fabsf(next[z][n]));
           }
