@@ -315,7 +315,7 @@ def run_ours(args) -> dict:
             tp_comm.close()
     import gc
 
-    del step, model
+    del step, model, job  # the job holds the model, its optimizer and its graphs too
     gc.collect()
     torch.cuda.empty_cache()
     if world == 1 and args.linear_quant == "bf16" and not args.no_fp8_variant:
