@@ -370,8 +370,11 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   TORCH_CHECK(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == B &&
                   lengths.is_contiguous() && lengths.device() == q.device(),
               "fp4_kv_attention: lengths must be a contiguous int32 vector of ", num(B), " on q's device");
-  TORCH_CHECK(table.size(1) * a.R <= INT32_MAX - 1024 && window >= 0 && window <= INT32_MAX && softcap >= 0,
-              "fp4_kv_attention: window and softcap must not be negative, a table less than 2^31 - 1024 rows wide");
+  TORCH_CHECK(table.size(1) * a.R + T <= INT32_MAX - 1024 && window >= 0 && softcap >= 0,
+              "fp4_kv_attention: window and softcap must not be negative, table rows and tokens below 2^31 - 1024");
+  // A window of the whole table sees what no window sees.  Positions, -T at the least, less a smaller
+  // window stay within 32 bits.
+  if (window >= table.size(1) * a.R) window = 0;
   if (sink.has_value())
     TORCH_CHECK(sink->scalar_type() == at::kFloat && sink->numel() == H && sink->is_contiguous() &&
                     sink->device() == q.device(), "fp4_kv_attention: sink must be ", num(H), " contiguous fp32 values");

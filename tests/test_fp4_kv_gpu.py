@@ -63,6 +63,16 @@ def test_attention_window_and_softcap(cuda, window):
     _attend_case(cuda, [1, 20, 100, 500], h=16, hk=1, d=128, rows=64, window=window, softcap=15.0, qscale=4.0)
 
 
+@pytest.mark.parametrize("room", [0, 40000])
+def test_attention_windows_wider_than_any_cache(cuda, room):
+    # less than t keys: the first queries' positions are negative, the window's lower end far below them
+    case = dict(h=16, hk=1, d=64, rows=16, t=40, room=room)
+    for lens in ([0, 1, 39, 40, 41], [3, 200]):
+        want = _attend_case(cuda, lens, **case)
+        for window in (2 ** 31 - 1, 2 ** 31 - 20, 2 ** 31):
+            assert torch.equal(_attend_case(cuda, lens, window=window, **case), want)
+
+
 def test_attention_sharp_and_flat_scores(cuda):
     _attend_case(cuda, [300, 1000], h=8, hk=2, d=128, rows=64, qscale=60.0)  # scores in the hundreds
     _attend_case(cuda, [300, 1000], h=8, hk=2, d=128, rows=64, qscale=1e-6)
