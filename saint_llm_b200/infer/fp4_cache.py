@@ -9,9 +9,10 @@ lengths and reference counts, all on the device:
 * ``fork`` makes sequences copies of others (pages shared, part-filled last pages copied), ``free``
   ends them, ``compact`` moves the pages in use to the front of the pool.
 
-At 4.25 bits a value a page takes 0.27 of its bf16 size.  Nothing is read on the host, so a step can
-be captured in a CUDA graph (``reserve`` works in place); what went wrong on the device -- no free
-page, an index out of range -- is raised by ``ops.gemm.check_errors``.
+At 4.25 bits a value a page takes 0.27 of its bf16 size.  Nothing is read on the host and the state
+keeps its addresses, so a step captured in a CUDA graph follows forks and compactions between its
+replays; what went wrong on the device -- no free page, an index out of range -- is raised by
+``ops.gemm.check_errors``.
 
 ``fp4_beam_search`` decodes sliding-window models with it: one prefill per prompt, a fork to all
 beams, then a reserve, one write and attention per layer, and a fork per step.
@@ -79,9 +80,10 @@ class Fp4KVCache:
 
     def fork(self, parents: Tensor | Sequence[int], children: Tensor | Sequence[int]) -> None:
         """Sequences ``children`` become copies of ``parents`` as they are now (-1: empty)."""
-        self.table, self.lengths, self.refcount = page_ops.fork_pages(
-            self.pool, self.table, self.lengths, self.refcount, self._ids(parents), self._ids(children),
-            page_rows=self.page_rows)
+        state = page_ops.fork_pages(self.pool, self.table, self.lengths, self.refcount, self._ids(parents),
+                                    self._ids(children), page_rows=self.page_rows)
+        for mine, new in zip((self.table, self.lengths, self.refcount), state, strict=True):
+            mine.copy_(new)
 
     def free(self, seqs: Tensor | Sequence[int]) -> None:
         ids = self._ids(seqs)
@@ -89,7 +91,9 @@ class Fp4KVCache:
 
     def compact(self) -> Tensor:
         """Pages in use to the front of the pool; returns how many there are (device scalar)."""
-        self.table, self.refcount, used = page_ops.compact_pages(self.pool, self.table, self.refcount)
+        table, refcount, used = page_ops.compact_pages(self.pool, self.table, self.refcount)
+        self.table.copy_(table)
+        self.refcount.copy_(refcount)
         return used
 
 

@@ -224,3 +224,55 @@ def test_decode_step_in_a_cuda_graph(cuda):
         assert torch.equal(out, step(b))
     assert torch.equal(a.table, b.table) and a.lengths.tolist() == [40, 40, 40]
     check_errors(cuda)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_state_keeps_its_addresses(device, request):
+    if device == "cuda":
+        request.getfixturevalue("cuda")
+    cache = Fp4KVCache(1, 8, max_seqs=3, max_len=64, head_dim=32, page_rows=16, device=device)
+    state = [cache.table, cache.lengths, cache.refcount]
+    where = [t.data_ptr() for t in state]
+    cache.reserve([1], 40)
+    cache.fork([1], [0])
+    cache.free([1])
+    cache.compact()
+    assert [t.data_ptr() for t in (cache.table, cache.lengths, cache.refcount)] == where
+    assert state[0].tolist() == [[0, 1, 2, -1], [-1] * 4, [-1] * 4] and state[1].tolist() == [40, 0, 0]
+    assert state[2].tolist() == [1, 1, 1, 0, 0, 0, 0, 0]
+
+
+@pytest.mark.gpu
+def test_captured_step_follows_forks_and_compaction(cuda):
+    from saint_llm_b200.ops.gemm import check_errors
+
+    gen = torch.Generator().manual_seed(8)
+    make = lambda: Fp4KVCache(1, 30, max_seqs=3, max_len=96, head_dim=64, page_rows=16, device=cuda)  # noqa: E731
+    a, b = make(), make()
+    seqs = torch.arange(3, dtype=torch.int32, device=cuda)
+    k, v = (torch.zeros(3, 1, 64, device=cuda, dtype=torch.bfloat16) for _ in range(2))
+    q = torch.zeros(3, 4, 1, 64, device=cuda, dtype=torch.bfloat16)
+
+    def step(cache):
+        cache.write(0, k, v, cache.reserve(seqs, 1))
+        return cache.attend(0, q)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):  # warm-up on another cache
+        step(make())
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(a)
+    for i in range(24):
+        for x in (k, v, q):
+            x.copy_(torch.randn(x.shape, generator=gen))
+        graph.replay()
+        assert torch.equal(out, step(b))
+        for cache in (a, b):
+            if i % 5 == 2:
+                cache.fork([2, 0], [0, 1])
+            if i % 7 == 3:
+                cache.compact()
+    assert torch.equal(a.table, b.table) and torch.equal(a.refcount, b.refcount)
+    check_errors(cuda)
