@@ -65,6 +65,9 @@ class Fp4KVCache:
 
     def read(self, layer: int, seq: int, length: int, *, dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
         """The first ``length`` K and V rows (length, kv_heads, head_dim) of a sequence."""
+        if not 0 <= seq < self.table.shape[0] or not 0 <= length <= self.table.shape[1] * self.page_rows:
+            raise IndexError(f"{length} rows of sequence {seq}: the cache has {self.table.shape[0]} sequences of up to "
+                             f"{self.table.shape[1] * self.page_rows}")
         pos = torch.arange(length, device=self.table.device)
         slots = self.table[seq, pos // self.page_rows].long() * self.page_rows + pos % self.page_rows
         return fp4_kv_read(self.pool[:, layer], slots, head_dim=self.head_dim, dtype=dtype)
@@ -75,7 +78,11 @@ class Fp4KVCache:
         table, lengths = self.table, self.lengths
         if seqs is not None:
             ids = self._ids(seqs).long()
-            table, lengths = table[ids], lengths[ids]
+            at = ids.clamp(0, table.shape[0] - 1)
+            if not ids.is_cuda and not torch.equal(ids, at):
+                raise IndexError(f"sequences {ids.tolist()} of {table.shape[0]}")
+            # on CUDA a length that no table holds records the error where the kernel reads it
+            table, lengths = table[at], torch.where(ids == at, lengths[at], torch.iinfo(torch.int32).max)
         return fp4_kv_attention(q, self.pool[:, layer], table, lengths, window=window, sink=sink, softcap=softcap)
 
     def fork(self, parents: Tensor | Sequence[int], children: Tensor | Sequence[int]) -> None:

@@ -276,3 +276,36 @@ def test_captured_step_follows_forks_and_compaction(cuda):
                 cache.compact()
     assert torch.equal(a.table, b.table) and torch.equal(a.refcount, b.refcount)
     check_errors(cuda)
+
+
+def test_sequences_out_of_range_are_refused():
+    cache = Fp4KVCache(1, 4, max_seqs=2, max_len=32, head_dim=32, page_rows=16)
+    cache.reserve([0, 1], 3)
+    q = torch.zeros(1, 2, 1, 32, dtype=torch.bfloat16)
+    for seqs in ([2], [-1], torch.tensor([5])):
+        with pytest.raises(IndexError):
+            cache.attend(0, q, seqs)
+    for seq, length in ((2, 1), (-1, 1), (0, 33), (0, -1)):
+        with pytest.raises(IndexError):
+            cache.read(0, seq, length)
+
+
+@pytest.mark.gpu
+def test_sequences_out_of_range_are_recorded(cuda):
+    from saint_llm_b200.ops.gemm import check_errors
+
+    cache = Fp4KVCache(1, 4, max_seqs=2, max_len=32, head_dim=32, page_rows=16, device=cuda)
+    gen = torch.Generator().manual_seed(2)
+    k = torch.randn(2, 3, 32, generator=gen).to(cuda)
+    cache.write(0, k, k, cache.reserve([0, 1], 3))
+    q = torch.randn(2, 4, 1, 32, generator=gen).to(cuda, torch.bfloat16)
+    good = cache.attend(0, q, [0, 1])
+    check_errors(cuda)
+    for wrong in (2, -1):
+        out = cache.attend(0, q, torch.tensor([0, wrong], device=cuda))
+        assert torch.equal(out[0], good[0])
+        with pytest.raises(RuntimeError, match="out of bounds"):
+            check_errors(cuda)
+    with pytest.raises(IndexError):
+        cache.read(0, 0, 33)
+    check_errors(cuda)
