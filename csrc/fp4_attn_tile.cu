@@ -129,7 +129,9 @@ __device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uin
   return make_int2(kbias, windows);
 }
 
-enum Barrier { kQFull, kKFull, kSFull, kPFull, kVFull, kOFull, kBarriers };
+// kReady: every softmax warp has seen kKFull of the tile.  Without it warp 0 and the operand warps could
+// complete kKFull once more before a warp that was held up looks, and a wait by parity would miss both.
+enum Barrier { kQFull, kKFull, kReady, kSFull, kPFull, kVFull, kOFull, kBarriers };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4AttnArgs a) {
@@ -387,7 +389,9 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
       for (int t = 0; t < count && alive; ++t) {
         const int key0 = key_begin + t * kKeys;
         wait(kKFull, n_tile);  // the operand warps' word on the tile
+        arrive(kReady);
         if (warp == 0) {
+          wait(kReady, n_tile);
           if (n_pv > 0) wait(kOFull, n_pv - 1);  // P lies where S goes
           if (alive && elect_one()) {
             tc_fence_after();

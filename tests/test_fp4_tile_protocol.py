@@ -1,0 +1,89 @@
+"""The waits of the many-row 4-bit attention kernel as a model on the CPU: its roles are stepped in
+random orders, some far slower than others, and no wait by parity may pass early or find its phase
+gone.  The steps are those of ``csrc/fp4_attn_tile.cu``."""
+
+import random
+
+import pytest
+
+
+class Barrier:
+    """An mbarrier: a phase completes when ``count`` arrivals are in; waits see its parity only."""
+
+    def __init__(self, count):
+        self.count, self.pending, self.phase = count, count, 0
+
+    def arrive(self):
+        self.pending -= 1
+        if self.pending == 0:
+            self.pending, self.phase = self.count, self.phase + 1
+
+    def passes(self, n):
+        assert self.phase < n + 2, f"the wait for completion {n} finds {self.phase} of them: its phase is gone"
+        if (self.phase ^ n) & 1:
+            assert self.phase == n + 1, f"the wait for completion {n} passes at {self.phase}"
+            return True
+        return False
+
+
+def _operands(bars, tiles):
+    """An operand warp: K when S of the tile before is done, V when its P V is."""
+    for n in range(tiles):
+        if n > 0:
+            yield "S", n - 1
+        bars["K"].arrive()
+        if n > 0:
+            yield "O", n - 1
+        bars["V"].arrive()
+
+
+def _softmax(bars, warp, tiles, meet):
+    """A softmax warp; the first one issues the products (which complete at once)."""
+    for n in range(tiles):
+        yield "K", n
+        if meet:
+            bars["ready"].arrive()
+        if warp == 0:
+            if meet:
+                yield "ready", n
+            if n > 0:
+                yield "O", n - 1
+            bars["S"].arrive()
+        yield "S", n
+        bars["P"].arrive()
+        if warp == 0:
+            yield "V", n
+            yield "P", n
+            bars["O"].arrive()
+    yield "O", tiles - 1
+
+
+def _run(seed, *, meet, tiles=5):
+    rng = random.Random(seed)
+    bars = {name: Barrier(1 if name in "SO" else 4) for name in ("K", "V", "P", "S", "O", "ready")}
+    roles = [_operands(bars, tiles) for _ in range(4)] + [_softmax(bars, w, tiles, meet) for w in range(4)]
+    speed = [rng.choice([1, 1, 100]) for _ in roles]
+    waits = {i: next(r) for i, r in enumerate(roles)}
+    for _ in range(20000):
+        i = rng.choices(list(waits), [speed[i] for i in waits])[0]
+        name, n = waits[i]
+        if bars[name].passes(n):
+            try:
+                waits[i] = next(roles[i])
+            except StopIteration:
+                del waits[i]
+                if not waits:
+                    return
+    raise AssertionError(f"still waiting: {waits}")
+
+
+def test_no_wait_misses_its_phase():
+    for seed in range(300):
+        _run(seed, meet=True)
+
+
+def test_the_model_finds_the_missing_meeting():
+    """Where softmax warps do not meet before S is issued, one that is held up loses a phase of K."""
+    with pytest.raises(AssertionError, match="phase is gone"):
+        for seed in range(300):
+            _run(seed, meet=False)
