@@ -564,6 +564,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t r[32];
+          __syncwarp();
           if (count > 0) {
             tmem_ld32(to + c * 32, r);
             tmem_ld_wait();
@@ -571,14 +572,15 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
 #pragma unroll
             for (int j = 0; j < 32; ++j) r[j] = 0;
           }
-          if (row >= rows) continue;
           const float add = (poison >> c) & 1u ? NAN : 0.f;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float o[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(r[8 * q + j]) * keep * power + add;
-            if (whole) {
+            if (row >= rows) {
+              // nothing to write; the lane stays, for the next turn's load is the whole warp's
+            } else if (whole) {
               Few<T, 8> y;
 #pragma unroll
               for (int j = 0; j < 8; ++j) y.v[j] = static_cast<T>(o[j]);
