@@ -161,14 +161,14 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = *tslot;
-  // The n-th completion of a barrier.  A wait that runs out records itself; the role then ends.
+  // The n-th completion of a barrier.  A wait that runs out records itself, and the warp (all of its lanes:
+  // what follows is done together) does nothing more; the operand warps, which meet at a named barrier,
+  // agree on that first.
   bool alive = true;
   auto wait = [&](int which, uint32_t n) {
-    if (alive && !mbar_wait(bar + which, n & 1, nullptr, 0)) {
-      record_error(a.err, kErrTimeoutAccum);
-      alive = false;
-    }
-    __syncwarp();
+    const bool done = alive && mbar_wait(bar + which, n & 1, nullptr, 0);  // errors of other kinds do not end it
+    if (alive && !done) record_error(a.err, kErrTimeoutAccum);
+    alive = __all_sync(0xffffffffu, done);
   };
   auto arrive = [&](int which) {  // one per warp
     __syncwarp();
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         load(key_begin);
         find(key_begin + kKeys);
       }
-      for (int t = 0; t < count && alive; ++t) {
+      for (int t = 0; t < count; ++t) {
         const int key0 = key_begin + t * kKeys;
         Tile& tile = tiles[n_tile & 1];
         bool ok = lost == 0;
@@ -278,7 +278,12 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           ok = ok && (!((seen >> x) & 1u) || ((k <= 1 || (k > 112 && k <= 140)) && (v <= 1 || (v > 112 && v <= 140))));
         }
         if (n_tile > 0) wait(kSFull, n_tile - 1);  // K is free
-        const bool plain = most_of(ok ? 0 : 1, red, part, lane) == 0 && !careful;
+        const int word = most_of(!alive ? 2 : ok ? 0 : 1, red, part, lane);
+        if (word == 2) {
+          alive = false;
+          break;
+        }
+        const bool plain = word == 0 && !careful;
         int kbias = 112, windows = 1;
         const bool scribe = part == 0 && lane == 0;
         if (!plain) {

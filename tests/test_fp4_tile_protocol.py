@@ -87,3 +87,45 @@ def test_the_model_finds_the_missing_meeting():
     with pytest.raises(AssertionError, match="phase is gone"):
         for seed in range(300):
             _run(seed, meet=False)
+
+
+class Meeting:
+    """A named barrier of four warps: a warp that arrives goes on when all four have."""
+
+    def __init__(self):
+        self.arrived, self.turns = 0, 0
+
+
+def _operand_loop(meeting, words, warp, fails_at, tiles, agree):
+    """An operand warp's turns, of which ``fails_at`` is the one where a wait of its runs out."""
+    alive = True
+    for n in range(tiles):
+        if not agree and not alive:
+            return
+        words[warp] = not alive
+        meeting.arrived += 1
+        turn = meeting.turns
+        if meeting.arrived == 4:
+            meeting.arrived, meeting.turns = 0, meeting.turns + 1
+            meeting.verdict = any(words)
+        while meeting.turns == turn:
+            yield
+        if agree and meeting.verdict:
+            return
+        if fails_at == n:
+            alive = False
+        yield
+
+
+def _ends(agree, late):
+    meeting, words = Meeting(), [False] * 4
+    roles = [_operand_loop(meeting, words, w, 2 if w == late else None, 6, agree) for w in range(4)]
+    for _ in range(200):
+        roles = [r for r in roles if next(r, "end") != "end"]
+    return not roles
+
+
+def test_operand_warps_end_together_when_a_wait_runs_out():
+    """One warp's wait runs out and the others' do not: none is left at the named barrier."""
+    assert all(_ends(True, late) for late in range(4))
+    assert not any(_ends(False, late) for late in range(4))  # as it would be if each left alone
