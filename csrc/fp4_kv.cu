@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kRowThreads) fp4_kv_write_kernel(const RowsArg
       // the magnitude is 1.m * 2^x: the exponent is x - 2 while 1.m <= 1.5
       const int e = max(-126, static_cast<int>(most >> 23) - 129 + ((most & 0x7fffffu) > 0x400000u ? 1 : 0));
       const uint32_t word = bad ? 0u : e2m1_codes<T>(f, __uint_as_float(static_cast<uint32_t>(127 - e) << 23));
-      uint8_t* slab = page[y] + head * a.slab;
+      uint8_t* slab = page[y] + static_cast<int64_t>(head) * a.slab;
       const int r = kv * a.R + in_page[y];
       *reinterpret_cast<uint32_t*>(slab + r * (D / 2) + part * 4) = word;
       if ((part & 3) == 0) slab[a.R * D + r * (D / 32) + part / 4] = static_cast<uint8_t>(bad ? 255 : e + 127);
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kRowThreads) fp4_kv_read_kernel(const RowsArgs
       word[y][u] = 0;
       byte[y][u] = 127;
       if (page != nullptr && unit0 + u < units) {
-        const uint8_t* slab = page + ((unit0 + u) >> 1) * a.slab;
+        const uint8_t* slab = page + static_cast<int64_t>((unit0 + u) >> 1) * a.slab;
         const int at = ((unit0 + u) & 1) * a.R + r;
         word[y][u] = *reinterpret_cast<const uint32_t*>(slab + at * (D / 2) + part * 4);
         byte[y][u] = slab[a.R * D + at * (D / 32) + part / 4];
