@@ -93,14 +93,15 @@ struct ReserveArgs {
 // One block: the pages that `count` more rows of each sequence open, in the order of the sequences;
 // all or nothing.  The pages' ids go into the table, the rows' slots out.
 __global__ void __launch_bounds__(kPlan) reserve_rows_kernel(const ReserveArgs a) {
-  // pages that sequence i needs, with its row and length; -1: out of range
+  // pages that sequence i needs, with its row and length; -1: out of range.  Rows and a page more take 32 bits.
+  const uint32_t more = static_cast<uint32_t>(a.R) - 1u;
   auto needs = [&](int i, int& row, int& len, int* err) {
     row = a.rows[i];
     len = 0;
     if (!index_ok(row, 0, a.S, err)) return -1;
     len = a.lengths[row];
     if (!index_ok(len, 0, static_cast<int64_t>(a.P) * a.R - a.count + 1, err)) return -1;
-    return (len + a.count + a.R - 1) / a.R - (len + a.R - 1) / a.R;
+    return static_cast<int>((static_cast<uint32_t>(len) + a.count + more) / a.R - (static_cast<uint32_t>(len) + more) / a.R);
   };
   int need = 0, bad = 0;
   for (int i0 = 0; i0 < a.n; i0 += kPlan) {
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(kPlan) reserve_rows_kernel(const ReserveArgs a
     const int first = before + block_scan(pages, &total);
     for (int x = 0; x < pages; ++x) {
       const int page = a.found[first + x];
-      a.table[static_cast<int64_t>(row) * a.P + (len + a.R - 1) / a.R + x] = page;
+      a.table[static_cast<int64_t>(row) * a.P + (static_cast<uint32_t>(len) + more) / a.R + x] = page;
       a.refcount[page] = 1;
     }
     before += total;
@@ -337,6 +338,12 @@ void launch_after(void (*kernel)(A), dim3 grid, const A& args, cudaStream_t stre
   C10_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args));
 }
 
+// The kernels count pages and sequences in 32 bits, and step past the last by a block's share.
+void check_counts(int64_t n_pages, int64_t sequences, int64_t forks, const char* who) {
+  TORCH_CHECK(std::max({n_pages, sequences, forks}) <= INT32_MAX - 4 * kPlan, who,
+              ": more pages or sequences than 32 bits count");
+}
+
 // The pool as pages of bytes; returns the bytes of a page.
 int64_t check_pool(const torch::Tensor& pool, const torch::Tensor& table, const torch::Tensor& refcount, const char* who) {
   TORCH_CHECK(pool.is_cuda() && pool.dim() >= 2 && pool.is_contiguous(), who,
@@ -347,8 +354,9 @@ int64_t check_pool(const torch::Tensor& pool, const torch::Tensor& table, const 
   TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous() &&
                   table.device() == pool.device(), who, ": table must be a contiguous (rows, pages) int32 tensor on the pool's device");
   TORCH_CHECK(refcount.scalar_type() == at::kInt && refcount.dim() == 1 && refcount.is_contiguous() &&
-                  refcount.device() == pool.device() && refcount.size(0) == pool.size(0) && pool.size(0) < INT32_MAX, who,
+                  refcount.device() == pool.device() && refcount.size(0) == pool.size(0), who,
               ": refcount must be a contiguous int32 vector of one count per page");
+  check_counts(pool.size(0), table.size(0), 0, who);
   return bytes;
 }
 
@@ -366,6 +374,7 @@ torch::Tensor reserve_rows(torch::Tensor table, torch::Tensor lengths, torch::Te
               "reserve_rows: lengths, refcount and rows must be contiguous int32 vectors on the table's device");
   TORCH_CHECK(count > 0 && page_rows > 0 && table.size(1) * page_rows <= INT32_MAX && count <= INT32_MAX / 2,
               "reserve_rows: count and page_rows must be positive");
+  check_counts(refcount.size(0), table.size(0), rows.size(0) * ((count + page_rows - 1) / page_rows), "reserve_rows");
   c10::cuda::CUDAGuard guard(table.device());
   auto slots = at::detail::empty_cuda({rows.size(0), count}, at::kLong, table.device(), std::nullopt);
   if (rows.size(0) == 0) return slots;
@@ -403,6 +412,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> fork_pages(torch::Tensor
   TORCH_CHECK(vec(parents, F) && vec(children, F),
               "fork_pages: parents and children must be contiguous int32 vectors of one length on the pool's device");
   TORCH_CHECK(page_rows > 0 && table.size(1) * page_rows <= INT32_MAX, "fork_pages: page_rows must be positive");
+  check_counts(0, 0, F, "fork_pages");
   c10::cuda::CUDAGuard guard(pool.device());
   if (F == 0) return {table.clone(), lengths.clone(), refcount.clone()};
   auto new_table = ints(table.sizes(), table), new_lengths = ints(lengths.sizes(), table), new_refs = ints(refcount.sizes(), table);
