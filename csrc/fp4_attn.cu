@@ -20,7 +20,8 @@
 // * q is scaled by a power of two per row to the top of fp16's range (bf16 keeps its 8 bits, what
 //   falls below 2^-38 of the row's largest is lost).  p is held times 2^15: fp16's 11 bits for
 //   weights down to 2^-29 of the largest.  A row's maximum is left as it is while the new one is at
-//   most 0.9 larger (log2), for which fp16 has room: the sums are rescaled less often.
+//   most 0.9 larger (log2), for which fp16 has room: the sums are rescaled less often.  (Above 2^16
+//   fp32 rounds that 0.9: no lag there, and the maximum is taken from the scores before 15 is added.)
 // * Operand order: dims and keys may be summed in any order, so a thread's operands are chosen to
 //   lie together: d/4 dims of a key for K; for V the d/16 bytes of its d/8 output dims, two keys'
 //   nibbles merged into the bytes that cvt turns into a pair.
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
       float acc[D / 16][NT][4];     // dims g d/8 + 2 x (elements 0, 1) and + 1 (2, 3), the same rows
       float poison[NT][2];          // NaN once a visible V block of this thread's dims was NaN
       int out_unit = 0;             // acc holds sums times 2^-out_unit
-      bool out_of_range = false;    // maxima above 2^16
+      bool out_of_range = false;    // maxima above kCoarse
 #pragma unroll
       for (int z = 0; z < NT; ++z) {
         m[z][0] = m[z][1] = -INFINITY;
@@ -455,14 +456,14 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
             float x = fmaxf(fmaxf(s[0][z][n], s[0][z][2 + n]), fmaxf(s[1][z][n], s[1][z][2 + n]));
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-            // fp16 holds p up to 2^15.99: the maximum may lag behind by 0.9
-            next[z][n] = x * f[z][n] > m[z][n] + 0.9f ? x * f[z][n] : m[z][n];
+            const float now = __fmul_rn(x, f[z][n]);
+            next[z][n] = now > m[z][n] + lag_of(now) ? now : m[z][n];
             moved = moved || next[z][n] != m[z][n];
             most = fmaxf(most, next[z][n] == -INFINITY ? 0.f : fabsf(next[z][n]));
           }
         }
         if (__any_sync(0xffffffffu, moved)) {
-          if (__any_sync(0xffffffffu, most > 65536.f)) out_of_range = true;
+          if (__any_sync(0xffffffffu, most > kCoarse)) out_of_range = true;
 #pragma unroll
           for (int z = 0; z < NT; ++z) {
             const float keep0 = shrink(m[z][0], next[z][0]), keep1 = shrink(m[z][1], next[z][1]);
@@ -480,15 +481,19 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           }
         }
         if (out_of_range) {
-          // the fused multiply-add below would keep the bits that rounding took from the maximum
-          each_score([&](float v, int, int z, int p) { return v * f[z][p & 1]; });
+          // The maximum is taken off first, from scores that were rounded as it was: 15 - m below would be rounded
+          // to the spacing of m, 16 - m from 2^24 on, and p would pass fp16's end.
+          each_score([&](float v, int, int z, int p) {
+            return __fsub_rn(__fmul_rn(v, f[z][p & 1]), m[z][p & 1] == -INFINITY ? 0.f : m[z][p & 1]);
+          });
           unit_factors();
         }
         // p times 2^15 (a row without a key so far keeps p = 0), as the B operand of the next product
         uint32_t p[2][NT][2];
 #pragma unroll
         for (int z = 0; z < NT; ++z) {
-          const float d0 = m[z][0] == -INFINITY ? 0.f : 15.f - m[z][0], d1 = m[z][1] == -INFINITY ? 0.f : 15.f - m[z][1];
+          const float d0 = out_of_range ? 15.f : m[z][0] == -INFINITY ? 0.f : 15.f - m[z][0];
+          const float d1 = out_of_range ? 15.f : m[z][1] == -INFINITY ? 0.f : 15.f - m[z][1];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
 #pragma unroll

@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
       float m = -INFINITY, l = 0.f;
       int unit = 0;                // this row's sums are held times 2^-unit
       uint32_t poison = 0;         // blocks of d whose sums are NaN
-      bool out_of_range = false;   // maxima above 2^16
+      bool out_of_range = false;   // maxima above kCoarse
       auto each_sum = [&](auto&& change) {  // of this row in TMEM
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         if (!plain) f = fmaxf(f * pow2f(tile.kbias - 112), 1.1754944e-38f);  // 0 would turn the mask's -inf into NaN
         const bool masked = key0 < inner_lo || key0 + kKeys > inner_hi, simple = !masked && plain;
         const float cap = a.softcap * kLog2e, squeeze = a.softcap > 0.f ? f * 2.f * kLog2e / a.softcap : 0.f;
-        auto capped = [&](float v) { return cap * (1.f - __fdividef(2.f, 1.f + ex2(v * squeeze))); };  // tanh x = 1 - 2 / (1 + e^2x)
+        auto capped = [&](float v) { return __fmul_rn(cap, 1.f - __fdividef(2.f, 1.f + ex2(v * squeeze))); };  // tanh x = 1 - 2 / (1 + e^2x)
         auto visible = [&](uint32_t raw, int j) {  // the raw score of key key0 + j, or -inf
           float v = __uint_as_float(raw);
           if (masked) v = key0 + j >= lo && key0 + j < hi ? v : -INFINITY;
@@ -445,10 +445,9 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           }
         }
         if (a.softcap > 0.f) most = most == -INFINITY ? most : capped(most);  // tanh keeps the order
-        else most *= f;
-        // fp16 holds p up to 2^15.99: the maximum may lag behind by 0.9
-        const float next = most > m + 0.9f ? most : m;
-        out_of_range = out_of_range || (next != -INFINITY && fabsf(next) > 65536.f);
+        else most = __fmul_rn(most, f);
+        const float next = most > m + lag_of(most) ? most : m;
+        out_of_range = out_of_range || (next != -INFINITY && fabsf(next) > kCoarse);
         if (t > 0 && __any_sync(0xffffffffu, next != m)) {
           const float keep = shrink(m, next);
           l *= keep;
@@ -458,7 +457,14 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           });
         }
         m = next;
-        const float d0 = m == -INFINITY ? 0.f : 15.f - m;  // p times 2^15
+        const float m0 = m == -INFINITY ? 0.f : m, d0 = m == -INFINITY ? 0.f : 15.f - m;  // p times 2^15
+        // For coarse maxima: taken off first, from scores that were rounded as they were (15 - m would be 16 - m from
+        // 2^24 on).  Capped scores may pass the maximum by their own rounding: fp16's end holds them.
+        auto below_maximum = [&](float v) {
+          const float x = __fsub_rn(v, m0);
+          return (x > 0.99f ? 0.99f : x) + 15.f;
+        };
+        const bool fine = simple && !__any_sync(0xffffffffu, out_of_range);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t r[32], h[16];
@@ -475,17 +481,15 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
             }
           };
           if (a.softcap > 0.f) {
-            if (simple) weigh([&](int j) { return capped(__uint_as_float(r[j])) + d0; });
+            if (fine) weigh([&](int j) { return capped(__uint_as_float(r[j])) + d0; });
             else weigh([&](int j) {
               const float v = visible(r[j], c * 32 + j);
-              return v == -INFINITY ? v : capped(v) + d0;
+              return v == -INFINITY ? v : below_maximum(capped(v));
             });
-          } else if (simple && !__any_sync(0xffffffffu, out_of_range)) {
+          } else if (fine) {
             weigh([&](int j) { return fmaf(__uint_as_float(r[j]), f, d0); });
           } else {
-            // the product rounded before the maximum is taken off: a fused one would keep the bits
-            // that rounding took from the maximum
-            weigh([&](int j) { return __fmul_rn(visible(r[j], c * 32 + j), f) + d0; });
+            weigh([&](int j) { return below_maximum(__fmul_rn(visible(r[j], c * 32 + j), f)); });
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_st16(ts + c * 16, h);  // over columns of S that have been read

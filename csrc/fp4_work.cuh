@@ -38,6 +38,11 @@ __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_ca
 // 2^(a - b) for a <= b, both possibly -inf
 __device__ __forceinline__ float shrink(float a, float b) { return a == b ? 1.f : ex2(a - b); }
 
+// Maxima above this are spaced by 2^-7 and more.  How far a row's maximum may lag behind the scores: fp16
+// holds p (times 2^15) up to 2^15.99, and 0.9 is 0.9 only where fp32 is fine enough.
+constexpr float kCoarse = 65536.f;
+__device__ __forceinline__ float lag_of(float score) { return fabsf(score) > kCoarse ? 0.f : 0.9f; }
+
 __device__ __forceinline__ float2 two_floats(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
 __device__ __forceinline__ float2 two_floats(uint32_t w, __nv_bfloat16) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));

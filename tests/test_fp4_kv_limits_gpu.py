@@ -57,3 +57,110 @@ def test_more_pages_than_32_bits_count_are_refused(cuda):
         fork_pages(pool, table, one, refs, one, one, page_rows=4)
     with pytest.raises(RuntimeError, match="32 bits"):
         reserve_rows(table, one, refs, one, 1, page_rows=4)
+
+
+# ----------------------------------------------------------------------------- attention
+BOTH = pytest.mark.parametrize("room", [0, 1 << 20], ids=["few_rows", "many_rows"])
+
+
+def _cache(cuda, k, v, rows, room):
+    """Pages with the rows k, v (N, heads, d) fp32 of one sequence, and a table wide enough for ``room`` keys
+    (with many query rows the tensor-core tiles run by then)."""
+    from saint_llm_b200.ops.fp4_kv import fp4_kv_slab_bytes, fp4_kv_write
+
+    n, hk, d = k.shape
+    count = -(-n // rows)
+    pages = torch.zeros(count, hk, fp4_kv_slab_bytes(rows, d), dtype=torch.uint8, device=cuda)
+    fp4_kv_write(k.to(cuda), v.to(cuda), pages, torch.arange(n, device=cuda))
+    table = torch.full((1, max(count, -(-room // rows))), -1, dtype=torch.int32, device=cuda)
+    table[0, :count] = torch.arange(count, dtype=torch.int32, device=cuda)
+    return pages, table, torch.tensor([n], dtype=torch.int32, device=cuda)
+
+
+def _definition(q, k, v, *, window=0, softcap=None, scale):
+    """(out, size, score, floor) in 64 bits, as the oracle's, for one sequence and K / V head; all of them by
+    dim: what a dim may be off by depends on that dim's values alone."""
+    _, h, t, d = q.shape
+    n = len(k)
+    pos = torch.arange(n - t, n, device=q.device).view(1, t, 1)
+    key = torch.arange(n, device=q.device)
+    seen = (key <= pos) & ((key > pos - window) if window else True)
+    k, v = k[:, 0], v[:, 0]
+    s = torch.einsum("htd,nd->htn", q[0].double(), k) * scale
+    size = torch.einsum("htd,nd->htn", q[0].double().abs(), k.abs()) * abs(scale)
+    if softcap:
+        s = softcap * torch.tanh(s / softcap)
+    s = torch.where(seen, s, float("-inf"))
+    p = torch.softmax(s, -1)
+    score = torch.where(p > 2.0 ** -45, size, 0.0).amax(-1, keepdim=True)  # an error matters where there is weight
+    floor = (torch.where(seen.unsqueeze(-1), v.abs(), 0.0).amax(2) * seen.sum(-1, keepdim=True)).expand(h, t, d)
+    return p @ v, p @ v.abs(), score, floor
+
+
+def _check(cuda, k, v, q, *, rows=32, room=0, extra=0.0, scale=1.0, blunt=False, **kw):
+    """k, v (N, 1, d) fp32, q (1, H, T, d) in 16 bits."""
+    from saint_llm_b200.ops.fp4_kv import fp4_kv_attention
+    from saint_llm_b200.ops.gemm import check_errors
+
+    pages, table, lengths = _cache(cuda, k, v, rows, room)
+    q = q.to(cuda)
+    got = fp4_kv_attention(q, pages, table, lengths, scale=scale, **kw)[0]
+    check_errors(cuda)
+    kk, vv = oracle.rows_of(pages, rows, q.shape[-1], torch.arange(len(k), device=cuda))
+    want, size, score, floor = _definition(q, kk, vv, scale=scale, **kw)
+    if blunt:  # scores so far apart, or V so alike, that the scores' own rounding does not show
+        score = torch.zeros_like(score)
+    allowed = oracle.bound(want, size, score, floor, q.dtype) + extra
+    err = (got.double() - want).abs()
+    assert bool((err <= allowed).all()), \
+        f"{float((err / allowed).nan_to_num(float('inf')).max()):.3g} of the bound, {int((~(err <= allowed)).sum())} of {err.numel()}"
+
+
+def _rand(gen, *shape):
+    return torch.randn(*shape, generator=gen)
+
+
+@BOTH
+@pytest.mark.parametrize("softcap", [None, 1e9])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_up_to_2_28_keep_their_weights(cuda, room, sign, softcap):
+    """Scores with no room for fractions, a unit or so apart within and between tiles.  All keys have
+    the same V, so whatever the weights, the output is V."""
+    gen = torch.Generator().manual_seed(3)
+    for low in (15, 20, 22, 24, 26):
+        q = torch.zeros(1, 16, 20, 64)
+        q[..., 0] = sign * 2.0 ** (low + 2 * torch.rand(1, 16, 20, generator=gen))
+        q[..., 1] = 0.2 + 1.6 * torch.rand(1, 16, 20, generator=gen)
+        k = torch.zeros(400, 1, 64)
+        k[:, 0, 0] = 1.0
+        k[:, 0, 1] = torch.randint(0, 3, (400,), generator=gen)
+        k[torch.randperm(400, generator=gen)[:100], 0, 0] = 0.5
+        v = torch.randint(1, 5, (1, 1, 64), generator=gen).float().expand(400, 1, 64)
+        _check(cuda, k, v, q.bfloat16(), room=room, softcap=softcap, blunt=True)
+        for n in (1, 2, 33, 129):
+            _check(cuda, k[:n], v[:n], q[:, :, :1].bfloat16(), softcap=softcap, blunt=True)
+
+
+def test_tiles_beside_other_work(cuda):
+    """The many-row kernel shares the GPU with other streams' kernels: warps are held up, results are not."""
+    from saint_llm_b200.ops.fp4_kv import fp4_kv_attention
+    from saint_llm_b200.ops.gemm import check_errors
+
+    gen = torch.Generator().manual_seed(11)
+    pages, table, lengths = oracle.filled([4096, 2500], hk=1, d=128, rows=64, gen=gen, device=cuda)
+    table = torch.nn.functional.pad(table, (0, 16384 - table.shape[1]), value=-1)
+    q = torch.randn(2, 16, 64, 128, generator=gen).to(cuda, torch.bfloat16)
+    want = fp4_kv_attention(q, pages, table, lengths)
+    x = torch.randn(1 << 24, generator=gen).to(cuda)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    outs = []
+    for i in range(40):
+        with torch.cuda.stream(streams[i % 4]):
+            if i % 4 < 2:
+                x * 1.5
+            else:
+                outs.append(fp4_kv_attention(q, pages, table, lengths))
+    torch.cuda.synchronize()
+    check_errors(cuda)
+    assert all(torch.equal(o, want) for o in outs)
