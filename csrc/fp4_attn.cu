@@ -351,8 +351,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           if (!plain) {
             khi = __reduce_max_sync(0xffffffffu, khi);
             vhi = __reduce_max_sync(0xffffffffu, vhi);
-            kbias = max(khi - 28, -14);
-            vbias = max(vhi - 28, 2);
+            kbias = max(khi - 28, kLeastBias);
+            vbias = max(vhi - 28, kLeastBias);
           }
 #pragma unroll
           for (int x = 0; x < C::kC; ++x) {
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           below = __reduce_max_sync(0xffffffffu, below);
           if (below == 0) break;
           most_byte = bias;
-          bias = below - 28;
+          bias = max(below - 28, kLeastBias);
         }
         if (!plain) {
           if (__any_sync(0xffffffffu, vnan)) {

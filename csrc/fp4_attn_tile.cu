@@ -30,7 +30,7 @@ constexpr int kThreads = 256;
 constexpr int kKeys = 128, kRows = 128;
 constexpr int kSegmentCost = 4;       // in tiles
 constexpr uint32_t kAtom = 16384;     // 128 rows x 128 bytes
-constexpr int kWindows = 10;          // 28 exponents each
+constexpr int kWindows = 10;          // 28 exponents each, from byte 254 down: -14 is the tenth's bias
 using List = Work<kKeys, kSegmentCost, kRows, 1>;
 
 // Operand descriptors, contracted over columns or over rows, and how far step s of 16 is from the
@@ -103,8 +103,8 @@ __device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uin
     if (k != 255) khi = max(khi, k);
     if (v != 255) vhi = max(vhi, v);
   }
-  const int kbias = max(most_of(khi, red, part, lane) - 28, -14);
-  int bias = max(most_of(vhi, red, part, lane) - 28, 2), windows = 1;
+  const int kbias = max(most_of(khi, red, part, lane) - 28, kLeastBias);
+  int bias = max(most_of(vhi, red, part, lane) - 28, kLeastBias), windows = 1;
   const bool scribe = part == 0 && lane == 0;
   if (scribe) tile.bias[0] = bias;
   while (windows < kWindows) {
@@ -115,7 +115,7 @@ __device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uin
     }
     below = most_of(below, red, part, lane);
     if (below == 0) break;
-    bias = below - 28;
+    bias = max(below - 28, kLeastBias);
     if (scribe) tile.bias[windows] = bias;
     ++windows;
   }

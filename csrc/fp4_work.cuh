@@ -77,10 +77,14 @@ __device__ __forceinline__ void scale_range(uint32_t word, int n, int& lo, int& 
   }
 }
 
-// fp16 bits of 2^(byte - bias - 15) for bytes in (bias, bias + 28], else 0.
+// The lowest window of exponents: its unit, 2^(bias - 112), is fp32's smallest power (2^-126), and every
+// byte up to 14 lies in it.
+constexpr int kLeastBias = -14;
+
+// fp16 bits of 2^(byte - bias - 15) for bytes in (bias, bias + 28], else 0; byte 0 is never written and reads as 0.
 __device__ __forceinline__ uint32_t scale_bits(int byte, int bias) {
   const uint32_t f = static_cast<uint32_t>(byte - bias);
-  return f <= 28u ? f << 10 : 0u;
+  return f <= 28u && byte != 0 ? f << 10 : 0u;
 }
 
 // The work as one list: for every sequence b, `row_tiles` (K / V head, Rows query rows) segments of

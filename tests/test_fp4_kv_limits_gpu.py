@@ -141,6 +141,19 @@ def test_scores_up_to_2_28_keep_their_weights(cuda, room, sign, softcap):
             _check(cuda, k[:n], v[:n], q[:, :, :1].bfloat16(), softcap=softcap, blunt=True)
 
 
+@BOTH
+@pytest.mark.parametrize("size", [1e-37, 2e-35, 3e-26, 3e-20])
+def test_values_down_to_the_smallest_scales(cuda, room, size):
+    """Scale bytes down to 2, alone and beside blocks and keys of other sizes."""
+    gen = torch.Generator().manual_seed(4)
+    for d, tiny in ((128, None), (64, 1e-37), (128, 2e-35)):
+        v = size * _rand(gen, 150, 1, d)
+        if tiny is not None:
+            v[:, :, 32:64] *= tiny / size
+            v[7, 0, :32] *= tiny / size
+        _check(cuda, _rand(gen, 150, 1, d), v, (0.3 * _rand(gen, 1, 8, 9, d)).bfloat16(), room=room)
+
+
 def test_tiles_beside_other_work(cuda):
     """The many-row kernel shares the GPU with other streams' kernels: warps are held up, results are not."""
     from saint_llm_b200.ops.fp4_kv import fp4_kv_attention
