@@ -343,6 +343,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
         } else {
           const int my_key = key0 + lane;
           if (!((halves >> (lane >> 4)) & 1u) || my_key < first || my_key >= last) kw = vw = 0x71717171u;  // nobody sees it
+          kw = without_zeros(kw, C::kC, buf + lane * (D / 2));
+          vw = without_zeros(vw, C::kC, buf + C::kCode + lane * (D / 2));
           int klo = 255, khi = 0, vlo = 255, vhi = 0;
           bool knan = false;
           scale_range(kw, C::kC, klo, khi, knan);
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
 #pragma unroll
           for (int x = 0; x < C::kC; ++x) {
             const int byte = (vw >> (8 * x)) & 255;
-            if (byte <= bias && byte > 1) below = max(below, byte);
+            if (byte <= bias) below = max(below, byte);
           }
           below = __reduce_max_sync(0xffffffffu, below);
           if (below == 0) break;

@@ -111,7 +111,7 @@ __device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uin
     int below = 0;  // the largest byte that no window holds yet
     for (int x = 0; x < C::kPasses; ++x) {
       const int v = (vbytes >> (8 * x)) & 255u;
-      if (((seen >> x) & 1u) && v <= bias && v > 1) below = max(below, v);
+      if (((seen >> x) & 1u) && v <= bias) below = max(below, v);
     }
     below = most_of(below, red, part, lane);
     if (below == 0) break;
@@ -273,9 +273,14 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         bool ok = lost == 0;
 #pragma unroll
         for (int x = 0; x < C::kPasses; ++x) {
-          const int k = static_cast<int>(kraw[x]), v = static_cast<int>(vraw[x]);
-          // exponents [-14, 13], or a block of zeros
-          ok = ok && (!((seen >> x) & 1u) || ((k <= 1 || (k > 112 && k <= 140)) && (v <= 1 || (v > 112 && v <= 140))));
+          if ((seen >> x) & 1u) {
+            const uint8_t* codes = rows_at[x / (C::kPasses / 2)] + x % (C::kPasses / 2) * C::kRowsAtOnce * (D / 2);
+            if (kraw[x] == 1 && zero_block(code[x])) kraw[x] = 0;
+            if (vraw[x] == 1 && zero_block(*reinterpret_cast<const uint4*>(codes + a.R * (D / 2)))) vraw[x] = 0;
+            const int k = static_cast<int>(kraw[x]), v = static_cast<int>(vraw[x]);
+            // exponents [-14, 13], or a block of zeros
+            ok = ok && (k == 0 || (k > 112 && k <= 140)) && (v == 0 || (v > 112 && v <= 140));
+          }
         }
         if (n_tile > 0) wait(kSFull, n_tile - 1);  // K is free
         const int word = most_of(!alive ? 2 : ok ? 0 : 1, red, part, lane);

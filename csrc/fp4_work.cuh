@@ -63,14 +63,25 @@ __device__ __forceinline__ float share_beside(float sink, float top, float l) {
   return mine / (mine + 32768.f);
 }
 
-// Extremes of the scale bytes of the tile's rows (NaN blocks and zero blocks, bytes 0 and 1, left out).
+// A block of zeros is written with the smallest scale, byte 1, which blocks of up to 6 * 2^-126 have too.
+__device__ __forceinline__ bool zero_block(uint4 codes) { return ((codes.x | codes.y | codes.z | codes.w) & 0x77777777u) == 0; }
+// A row's scale bytes, 0 for its blocks of zeros.
+__device__ __forceinline__ uint32_t without_zeros(uint32_t word, int n, const uint8_t* codes) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n && ((word >> (8 * i)) & 255u) == 1u && zero_block(*reinterpret_cast<const uint4*>(codes + 16 * i)))
+      word &= ~(255u << (8 * i));
+  return word;
+}
+
+// Extremes of the scale bytes of a row (NaN blocks, and zero blocks as byte 0, left out).
 __device__ __forceinline__ void scale_range(uint32_t word, int n, int& lo, int& hi, bool& nan) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (i >= n) break;
     const int b = (word >> (8 * i)) & 255;
     if (b == 255) nan = true;
-    else if (b > 1) {
+    else if (b > 0) {
       lo = min(lo, b);
       hi = max(hi, b);
     }

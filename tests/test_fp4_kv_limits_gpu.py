@@ -154,6 +154,20 @@ def test_values_down_to_the_smallest_scales(cuda, room, size):
         _check(cuda, _rand(gen, 150, 1, d), v, (0.3 * _rand(gen, 1, 8, 9, d)).bfloat16(), room=room)
 
 
+@BOTH
+def test_blocks_of_the_smallest_scale_are_no_zeros(cuda, room):
+    """Scale byte 1: magnitudes up to 6 * 2^-126, which a block of zeros has too."""
+    gen = torch.Generator().manual_seed(5)
+    small = lambda *shape: torch.randint(-6, 7, shape, generator=gen) * 2.0 ** -126  # noqa: E731
+    for d in (64, 128):
+        q = (0.3 * _rand(gen, 1, 8, 9, d)).bfloat16()
+        v = small(100, 1, d)
+        _check(cuda, _rand(gen, 100, 1, d), v, q, room=room)
+        q = torch.zeros(1, 8, 9, d)
+        q[..., 5], q[..., 40] = 2.0 ** 125 * torch.randint(-3, 4, (2, 1, 8, 9), generator=gen)
+        _check(cuda, small(100, 1, d), _rand(gen, 100, 1, d), q.bfloat16(), room=room)
+
+
 def test_tiles_beside_other_work(cuda):
     """The many-row kernel shares the GPU with other streams' kernels: warps are held up, results are not."""
     from saint_llm_b200.ops.fp4_kv import fp4_kv_attention
