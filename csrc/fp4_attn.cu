@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
             }
         } else {
           const int my_key = key0 + lane;
-          if (!((halves >> (lane >> 4)) & 1u) || my_key < first || my_key >= last) kw = vw = 0x71717171u;  // nobody sees it
+          if (!((halves >> (lane >> 4)) & 1u) || my_key < first || my_key >= last) kw = vw = 0;  // nobody sees it: a row of zeros
           kw = without_zeros(kw, C::kC, buf + lane * (D / 2));
           vw = without_zeros(vw, C::kC, buf + C::kCode + lane * (D / 2));
           int klo = 255, khi = 0, vlo = 255, vhi = 0;

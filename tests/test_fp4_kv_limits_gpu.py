@@ -168,6 +168,18 @@ def test_blocks_of_the_smallest_scale_are_no_zeros(cuda, room):
         _check(cuda, small(100, 1, d), _rand(gen, 100, 1, d), q.bfloat16(), room=room)
 
 
+@BOTH
+@pytest.mark.parametrize("size", [2.0 ** -45, 2.0 ** -100, 2.0 ** 60])
+def test_keys_of_other_sizes_in_part_filled_tiles(cuda, room, size):
+    """What lies beside the keys of a tile has no say in their unit."""
+    gen = torch.Generator().manual_seed(13)
+    for n in (2, 31, 100):
+        q = (_rand(gen, 1, 8, 9 if n > 9 else 2, 64) / size).bfloat16()
+        k = size * _rand(gen, n, 1, 64)
+        _check(cuda, k, _rand(gen, n, 1, 64), q, room=room)
+        _check(cuda, k, _rand(gen, n, 1, 64), q[:, :, -1:], window=20)
+
+
 def test_tiles_beside_other_work(cuda):
     """The many-row kernel shares the GPU with other streams' kernels: warps are held up, results are not."""
     from saint_llm_b200.ops.fp4_kv import fp4_kv_attention
