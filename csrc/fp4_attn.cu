@@ -15,8 +15,7 @@
 //   empty.  Codes become fp16 pairs with cvt.e2m1x2, exact.
 // * K and V scales are powers of two, applied to the fp16 pairs: exact while the exponent is in
 //   [-14, 13].  A tile with scales outside takes other exponents for K (28 from its own largest
-//   down) and runs its V product once per window of 28 exponents, the sums moved from unit to
-//   unit by powers of two.
+//   down) and runs its V product once per window of 28 exponents, each added to the sums in fp32.
 // * q is scaled by a power of two per row to the top of fp16's range (bf16 keeps its 8 bits, what
 //   falls below 2^-38 of the row's largest is lost).  p is held times 2^15: fp16's 11 bits for
 //   weights down to 2^-29 of the largest.  A row's maximum is left as it is while the new one is at
@@ -83,29 +82,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-// The sums' unit moved from 2^from to 2^to: exact but for what leaves fp32's range at the small
-// end.  Towards smaller units only as far as the largest sum stays finite; returns the unit.
-template <int N, int NT>
-__device__ __forceinline__ int to_unit(float (&acc)[N][NT][4], int from, int to) {
-  float big = 0.f;
-#pragma unroll
-  for (int x = 0; x < N; ++x)
-#pragma unroll
-    for (int z = 0; z < NT; ++z)
-#pragma unroll
-      for (int y = 0; y < 4; ++y) big = fmaxf(big, fabsf(acc[x][z][y]));
-  const int top = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23) - 127;
-  const int up = min(min(from - to, 126), max(0, 96 - top));
-  const float f = pow2f(max(up, -126)), again = pow2f(max(min(up + 126, 0), -126));
-#pragma unroll
-  for (int x = 0; x < N; ++x)
-#pragma unroll
-    for (int z = 0; z < NT; ++z)
-#pragma unroll
-      for (int y = 0; y < 4; ++y) acc[x][z][y] = acc[x][z][y] * f * again;
-  return from - up;
-}
-
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_rows_kernel(const Fp4AttnArgs a) {
   using C = Cfg<D, NT>;
@@ -263,7 +239,9 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
       float m[NT][2], sums[NT][4];  // maximum and sum of p (elements 0, 1) of rows 8 z + 2 c + x
       float acc[D / 16][NT][4];     // dims g d/8 + 2 x (elements 0, 1) and + 1 (2, 3), the same rows
       float poison[NT][2];          // NaN once a visible V block of this thread's dims was NaN
-      int out_unit = 0;             // acc holds sums times 2^-out_unit
+      int out_unit = 0;             // acc holds sums times 2^-out_unit: 0 or kLargeUnit
+      float kept[D / 16 * NT * 4];  // the sums, while acc takes a window's product
+      asm volatile("" ::"l"(kept) : "memory");  // in memory, not in registers that all tiles would miss
       bool out_of_range = false;    // maxima above kCoarse
 #pragma unroll
       for (int z = 0; z < NT; ++z) {
@@ -311,7 +289,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
         const uint32_t low = ((k16 - 0x01010101u) & (v16 - 0x01010101u) & 0x80808080u) ^ 0x80808080u;
         const bool inner = halves == 3u && key0 >= first && key0 + kTile <= last;  // every row was written
         bool plain = true, vnan = false;
-        int kbias = 112, vbias = 112;
+        int kbias = 112, vbias = 112, vhi = 0;
         uint32_t ksc[4], vsc[2][2];
         const int pair_at = (lane & ~7) | ((lane & 3) * 2) | ((lane >> 2) & 1);  // keys c and c + 4 side by side
         auto put_v_scales = [&](int bias, int most) {  // of the blocks whose byte is `most` or less
@@ -345,7 +323,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           if (!((halves >> (lane >> 4)) & 1u) || my_key < first || my_key >= last) kw = vw = 0;  // nobody sees it: a row of zeros
           kw = without_zeros(kw, C::kC, buf + lane * (D / 2));
           vw = without_zeros(vw, C::kC, buf + C::kCode + lane * (D / 2));
-          int klo = 255, khi = 0, vlo = 255, vhi = 0;
+          int klo = 255, khi = 0, vlo = 255;
           bool knan = false;
           scale_range(kw, C::kC, klo, khi, knan);
           scale_range(vw, C::kC, vlo, vhi, vnan);
@@ -544,24 +522,33 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
             }
           }
         };
-        // Ordinarily one product.  Else one for each window of 28 exponents, the largest first, the sums
-        // in the unit of each.
+        // Ordinarily one product, onto the sums.  Else one for each window of 28 exponents, the largest first, by
+        // itself: no size of one block, key or row limits another's.
         const bool windows = !plain || out_unit != 0;
         int bias = vbias, most_byte = 254;
+        auto each_sum = [&](auto&& change) {
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+            for (int z = 0; z < NT; ++z)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) acc[x][z][y] = change(acc[x][z][y], (x * NT + z) * 4 + y);
+        };
+        if (!plain && vhi > kLargeByte && out_unit == 0) {
+          out_unit = kLargeUnit;
+          each_sum([&](float v, int) { return v * pow2f(-kLargeUnit); });
+        }
         while (true) {
-          bool limited = false;
-          if (windows) {
-            const int got = out_unit = to_unit(acc, out_unit, bias - 112);
-            limited = got != bias - 112;
-            if (limited || bias != vbias) {
-              __syncwarp();
-              put_v_scales(got + 112, most_byte);
-              __syncwarp();
-              get_v_scales();
-            }
-          }
+          if (windows)
+            each_sum([&](float v, int at) {
+              kept[at] = v;
+              return 0.f;
+            });
           add_values();
-          if (plain || limited) break;
+          if (!windows) break;
+          const Power unit(bias - 112 - out_unit);
+          each_sum([&](float v, int at) { return unit.add(v, kept[at]); });
+          if (plain) break;
           int below = 0;  // the largest byte that no window has held yet
 #pragma unroll
           for (int x = 0; x < C::kC; ++x) {
@@ -572,6 +559,10 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           if (below == 0) break;
           most_byte = bias;
           bias = max(below - 28, kLeastBias);
+          __syncwarp();
+          put_v_scales(bias, most_byte);
+          __syncwarp();
+          get_v_scales();
         }
         if (!plain) {
           if (__any_sync(0xffffffffu, vnan)) {
@@ -602,7 +593,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           for (int n = 0; n < 2; ++n) ml[warp * C::kRows + 8 * z + 2 * c + n] = make_float2(m[z][n], sums[z][n]);
       }
       __syncthreads();
-      const float unit = pow2f(max(-126, min(126, out_unit)));
+      const float unit = pow2f(out_unit);
       float top[NT][2], whole_l[NT][2];
 #pragma unroll
       for (int z = 0; z < NT; ++z) {

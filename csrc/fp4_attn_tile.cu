@@ -17,8 +17,8 @@
 //   as 64-column 128B-swizzled atoms, V contracted over its rows.
 //
 // A tile with other exponents takes K's from its own largest 28 down, and runs P V once per window
-// of 28 exponents, each row's sums moved from unit to unit by powers of two; a row whose sums are
-// too large to follow to a small unit has no use for what is 2^-126 of them.
+// of 28 exponents, 64 dims at a time into the half of S that P leaves free; the softmax warps add that to
+// O in fp32.
 #include "fp4_work.cuh"
 
 namespace sv4 {
@@ -61,7 +61,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 
 // What the operand warps say about a tile.
 struct Tile {
-  int plain;   // all exponents in [-14, 13] and every page there
+  int plain;   // all exponents in [-14, 13] and every page there, O in units of 1
+  int large;   // O is held in units of 2^kLargeUnit
   int kbias;   // K's scales are 2^(byte - kbias - 15)
   int windows; // products P V
   int bias[kWindows];
@@ -89,7 +90,8 @@ __device__ __forceinline__ int most_of(int v, int* red, int part, int lane) {
 }
 
 // A tile with exponents outside [-14, 13], NaN blocks or missing keys: K's bias, V's windows and the
-// keys' marks, from the scale bytes (one per pass) of all operand threads.  Returns {kbias, windows}.
+// keys' marks, from the scale bytes (one per pass) of all operand threads.  Returns kbias, and the windows with
+// 256 added for V scales above kLargeByte.
 // Not inlined: its registers would be taken from every tile.
 template <int D>
 __device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uint32_t vbytes, uint32_t seen, uint32_t lost,
@@ -104,7 +106,8 @@ __device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uin
     if (v != 255) vhi = max(vhi, v);
   }
   const int kbias = max(most_of(khi, red, part, lane) - 28, kLeastBias);
-  int bias = max(most_of(vhi, red, part, lane) - 28, kLeastBias), windows = 1;
+  vhi = most_of(vhi, red, part, lane);
+  int bias = max(vhi - 28, kLeastBias), windows = 1;
   const bool scribe = part == 0 && lane == 0;
   if (scribe) tile.bias[0] = bias;
   while (windows < kWindows) {
@@ -126,12 +129,12 @@ __device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uin
     if (((seen >> x) & 1u) && ((vbytes >> (8 * x)) & 255u) == 255u) atomicOr(tile.nan_keys + row, 1u << blk);
     if ((lost >> x) & 1u) atomicOr(tile.nan_keys + row, 0x80000000u);
   }
-  return make_int2(kbias, windows);
+  return make_int2(kbias, windows + (vhi > kLargeByte ? 256 : 0));
 }
 
 // kReady: every softmax warp has seen kKFull of the tile.  Without it warp 0 and the operand warps could
 // complete kKFull once more before a warp that was held up looks, and a wait by parity would miss both.
-enum Barrier { kQFull, kKFull, kReady, kSFull, kPFull, kVFull, kOFull, kBarriers };
+enum Barrier { kQFull, kKFull, kReady, kSFull, kPFull, kVFull, kTFull, kOFull, kBarriers };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4AttnArgs a) {
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
   List list;
   if (!list.begin(a, row_tiles)) return;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBarriers; ++i) mbar_init(bar + i, i == kSFull || i == kOFull ? 1 : 4);
+    for (int i = 0; i < kBarriers; ++i) mbar_init(bar + i, i == kSFull || i == kTFull || i == kOFull ? 1 : 4);
     fence_barrier_init();
   }
   if (warp == 0) {
@@ -174,8 +177,9 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
     __syncwarp();
     if (lane == 0) mbar_arrive(bar + which);
   };
-  // Every role counts the same: segments, tiles and P V products so far.
-  uint32_t n_seg = 0, n_tile = 0, n_pv = 0;
+  // Every role counts the same: segments, tiles and P V windows so far; the softmax warps also what they
+  // let P be read for, and the products beside O.
+  uint32_t n_seg = 0, n_tile = 0, n_pv = 0, n_p = 0, n_t = 0;
 
   while (true) {
     const int take = list.take(), from_tile = list.from_tile(), b = list.b;
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           }
         }
       };
-      bool careful = false;  // a tile of this segment had other exponents: its sums have units
+      bool large = false;  // a tile of this segment had such V scales: its O has another unit
       if (count > 0) {
         find(key_begin);
         load(key_begin);
@@ -288,11 +292,10 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           alive = false;
           break;
         }
-        const bool plain = word == 0 && !careful;
+        const bool plain = word == 0 && !large;
         int kbias = 112, windows = 1;
         const bool scribe = part == 0 && lane == 0;
         if (!plain) {
-          careful = true;
           uint32_t kbytes = 0, vbytes = 0;
 #pragma unroll
           for (int x = 0; x < C::kPasses; ++x) {
@@ -301,10 +304,12 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           }
           const int2 found = describe<D>(tile, red, kbytes, vbytes, seen, lost, part, lane);
           kbias = found.x;
-          windows = found.y;
+          windows = found.y & 255;
+          large = large || found.y >= 256;
         }
         if (scribe) {
           tile.plain = plain;
+          tile.large = large;
           tile.kbias = kbias;
           tile.windows = windows;
         }
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
     } else {
       // ============================================================ softmax
       constexpr uint32_t kIdS = make_idesc_f16(128, 128, 0, 0, false, false);
-      constexpr uint32_t kIdO = make_idesc_f16(128, D, 0, 0, false, true);
+      constexpr uint32_t kIdO = make_idesc_f16(128, D, 0, 0, false, true), kIdT = make_idesc_f16(128, 64, 0, 0, false, true);
       const uint64_t dq = desc_cols(smem_u32(sq)), dk = desc_cols(smem_u32(sk)), dv = desc_rows(smem_u32(sv));
       const int row = threadIdx.x;  // of the tile; the warp's TMEM lanes
       const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16, ts = tbase + lanes, to = tbase + 128 + lanes;
@@ -382,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
       }
 
       float m = -INFINITY, l = 0.f;
-      int unit = 0;                // this row's sums are held times 2^-unit
+      int unit = 0;                // O holds sums times 2^-unit: 0 or kLargeUnit
       uint32_t poison = 0;         // blocks of d whose sums are NaN
       bool out_of_range = false;   // maxima above kCoarse
       auto each_sum = [&](auto&& change) {  // of this row in TMEM
@@ -399,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
       for (int t = 0; t < count && alive; ++t) {
         const int key0 = key_begin + t * kKeys;
         wait(kKFull, n_tile);  // the operand warps' word on the tile
+        tc_fence_before();  // what S overwrites has been read
         arrive(kReady);
         if (warp == 0) {
           wait(kReady, n_tile);
@@ -501,65 +507,63 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         }
         tmem_st_wait();
 
-        bool dropped = false;  // this row's sums are too large for smaller units
-        const int windows = tile.windows;
-        for (int w = 0; w < windows && alive; ++w) {
-          if (!plain) {
-            if (w > 0) {
-              wait(kOFull, n_pv - 1);
-              tc_fence_after();
-            } else {
-              for (int j = 0; j < kKeys; ++j)
-                if (key0 + j >= lo && key0 + j < hi) poison |= tile.nan_keys[j] & 0xfu;
-            }
-            // the row's sums to the unit of this window
-            const int want = tile.bias[w] - 112;
-            const bool sums = t > 0 || w > 0;
-            float big = 0.f;
-            if (sums)
-              each_sum([&](uint32_t (&r)[32]) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) big = fmaxf(big, fabsf(__uint_as_float(r[j])));
-              });
-            if (big == 0.f) unit = want;  // nothing to move
-            const int top = static_cast<int>(__float_as_uint(big) >> 23) - 127;
-            if (unit - want > min(126, max(0, 96 - top))) dropped = true;
-            const int by = dropped ? 0 : unit - want;
-            const float s0 = pow2f(max(by, -126)), s1 = pow2f(max(min(by + 126, 0), -126));
-            if (sums)
-              each_sum([&](uint32_t (&r)[32]) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * s0 * s1);
-              });
-            unit -= by;
-            if (__any_sync(0xffffffffu, dropped)) {  // such a row's P becomes 0, the others' stay
-#pragma unroll 1
-              for (int c = 0; c < 2; ++c) {
-                uint32_t r[32];
-                tmem_ld32(ts + c * 32, r);
-                tmem_ld_wait();
-#pragma unroll
-                for (int j = 0; j < 32; ++j) r[j] = dropped ? 0u : r[j];
-                tmem_st32(ts + c * 32, r);
-              }
-              tmem_st_wait();
-            }
-          }
+        // The product of window w (its V is complete), into O or, for 64 dims at `half`, beside P.
+        auto multiply = [&](bool beside, int half) {
           tc_fence_before();
           arrive(kPFull);
           if (warp == 0) {
             wait(kVFull, n_pv);
-            wait(kPFull, n_pv);
+            wait(kPFull, n_p);
             if (alive && elect_one()) {
               tc_fence_after();
 #pragma unroll
               for (int s = 0; s < kKeys / 16; ++s)
-                mma_f16_ts(tbase + 128, tbase + 8 * s, dv + step_rows(s), kIdO, t > 0 || w > 0 || s > 0 ? 1u : 0u);
-              mma_commit(bar + kOFull);
+                mma_f16_ts(tbase + (beside ? 64 : 128), tbase + 8 * s, dv + (half * kAtom >> 4) + step_rows(s),
+                           beside ? kIdT : kIdO, beside ? s > 0 : t > 0 || s > 0);
+              if (beside) mma_commit(bar + kTFull);
+              if (!beside || half == C::kAtoms - 1) mma_commit(bar + kOFull);
             }
             __syncwarp();
           }
+          ++n_p;
+        };
+        if (plain) {
+          multiply(false, 0);
           ++n_pv;
+        } else {
+          for (int j = 0; j < kKeys; ++j)
+            if (key0 + j >= lo && key0 + j < hi) poison |= tile.nan_keys[j] & 0xfu;
+          if (tile.large && unit == 0) {
+            unit = kLargeUnit;
+            if (t > 0)
+              each_sum([&](uint32_t (&r)[32]) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * pow2f(-kLargeUnit));
+              });
+          }
+          const int windows = tile.windows;
+          for (int w = 0; w < windows && alive; ++w) {
+            const Power power(tile.bias[w] - 112 - unit);
+            const bool first = t == 0 && w == 0;
+            for (int half = 0; half < C::kAtoms && alive; ++half) {
+              multiply(true, half);
+              wait(kTFull, n_t++);
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < 2; ++c) {
+                uint32_t r[32], o[32];
+                tmem_ld32(ts + 64 + c * 32, r);
+                tmem_ld32(to + half * 64 + c * 32, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  o[j] = __float_as_uint(power.add(__uint_as_float(r[j]), first ? 0.f : __uint_as_float(o[j])));
+                tmem_st32(to + half * 64 + c * 32, o);
+              }
+              tmem_st_wait();
+            }
+            ++n_pv;
+          }
         }
         ++n_tile;
       }
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         const bool whole = list.whole();
         const int i = row0 + row, h = head * G + min(i, G * a.T - 1) % G;
         const float keep = (l == 0.f ? 0.f : 1.f / l) * (whole && a.sink != nullptr ? share_beside(a.sink[h], m, l) : 1.f);
-        const float power = pow2f(max(-126, min(126, unit)));
+        const float power = pow2f(unit);
         const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.T + i / G, slot = list.part_row() + row;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {

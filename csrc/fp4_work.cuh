@@ -92,6 +92,17 @@ __device__ __forceinline__ void scale_range(uint32_t word, int n, int& lo, int& 
 // byte up to 14 lies in it.
 constexpr int kLeastBias = -14;
 
+// Windows are added to the sums in fp32, in units of 1, or of 2^kLargeUnit from the first tile on that has a
+// V scale above kLargeByte: with 2^24 keys and p up to 2^16 sums stay below 2^122 either way.  Beside such
+// values (2^79 and up) what is below 2^-110 is lost.
+constexpr int kLargeByte = 206, kLargeUnit = 48;
+// x 2^e + y for e in [-252, 127]
+struct Power {
+  float a, b;
+  __device__ __forceinline__ explicit Power(int e) : a(pow2f(max(e, -126))), b(pow2f(max(min(e + 126, 0), -126))) {}
+  __device__ __forceinline__ float add(float x, float y) const { return fmaf(x * a, b, y); }
+};
+
 // fp16 bits of 2^(byte - bias - 15) for bytes in (bias, bias + 28], else 0; byte 0 is never written and reads as 0.
 __device__ __forceinline__ uint32_t scale_bits(int byte, int bias) {
   const uint32_t f = static_cast<uint32_t>(byte - bias);

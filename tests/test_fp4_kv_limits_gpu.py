@@ -169,6 +169,16 @@ def test_blocks_of_the_smallest_scale_are_no_zeros(cuda, room):
 
 
 @BOTH
+def test_blocks_of_the_smallest_scale_beside_ordinary_ones(cuda, room):
+    gen = torch.Generator().manual_seed(12)
+    for d in (64, 128):
+        q, v = (0.3 * _rand(gen, 1, 8, 9, d)).bfloat16(), _rand(gen, 100, 1, d)
+        v[:, :, 32:64] = torch.randint(-6, 7, (100, 1, 32), generator=gen) * 2.0 ** -126
+        v[50:, :, :32] = 0.0
+        _check(cuda, _rand(gen, 100, 1, d), v, q, room=room)
+
+
+@BOTH
 @pytest.mark.parametrize("size", [2.0 ** -45, 2.0 ** -100, 2.0 ** 60])
 def test_keys_of_other_sizes_in_part_filled_tiles(cuda, room, size):
     """What lies beside the keys of a tile has no say in their unit."""
@@ -178,6 +188,37 @@ def test_keys_of_other_sizes_in_part_filled_tiles(cuda, room, size):
         k = size * _rand(gen, n, 1, 64)
         _check(cuda, k, _rand(gen, n, 1, 64), q, room=room)
         _check(cuda, k, _rand(gen, n, 1, 64), q[:, :, -1:], window=20)
+
+
+@BOTH
+@pytest.mark.parametrize("apart", [50, 80, 120, 160])
+def test_blocks_of_v_of_very_different_size(cuda, room, apart):
+    """Each block of 32 dims is as near as if it were alone, whatever the others' and the other keys' size."""
+    gen = torch.Generator().manual_seed(6)
+    for d in (64, 128):
+        q, k = (0.3 * _rand(gen, 1, 8, 9, d)).bfloat16(), _rand(gen, 300, 1, d)
+        v = _rand(gen, 300, 1, d)
+        v[:, :, :32] *= 2.0 ** (apart // 2)
+        v[:, :, -32:] *= 2.0 ** -((apart + 1) // 2)
+        _check(cuda, k, v, q, room=room)
+        v = _rand(gen, 300, 1, d) * 2.0 ** torch.randint(-apart // 2, apart // 2 + 1, (300, d // 32), generator=gen) \
+            .repeat_interleave(32, -1).view(300, 1, d)
+        _check(cuda, k, v, (40 * q.float()).bfloat16(), room=room)
+
+
+@BOTH
+def test_values_at_the_type_s_end_reach_only_the_rows_that_see_them(cuda, room):
+    """Keys that earlier rows of the same tile see and later ones do not hold the largest values.  What a row
+    beside them loses is 2^-110, however small its own values."""
+    gen = torch.Generator().manual_seed(7)
+    big = torch.finfo(torch.bfloat16).max * 0.7
+    for d in (64, 128):
+        q, k, v = (0.3 * _rand(gen, 1, 8, 9, d)).bfloat16(), _rand(gen, 300, 1, d), _rand(gen, 300, 1, d)
+        v[241:246] = big * torch.randint(-1, 2, (5, 1, d), generator=gen)
+        _check(cuda, k, v, q, room=room, window=52, extra=2.0 ** -110)
+        v[:] *= 2.0 ** -60
+        v[241:246] *= 2.0 ** 60
+        _check(cuda, k, v, q, room=room, window=52, extra=2.0 ** -110)
 
 
 def test_tiles_beside_other_work(cuda):

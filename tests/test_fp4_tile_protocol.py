@@ -27,54 +27,68 @@ class Barrier:
 
 
 def _operands(bars, tiles):
-    """An operand warp: K when S of the tile before is done, V when its P V is."""
-    for n in range(tiles):
+    """An operand warp: K when S of the tile before is done, V of a window when the P V before is.
+    ``tiles``: 0 for an ordinary tile, else the windows that its V takes."""
+    n_pv = 0
+    for n, windows in enumerate(tiles):
         if n > 0:
             yield "S", n - 1
         bars["K"].arrive()
-        if n > 0:
-            yield "O", n - 1
-        bars["V"].arrive()
+        for _ in range(max(1, windows)):
+            if n_pv > 0:
+                yield "O", n_pv - 1
+            bars["V"].arrive()
+            n_pv += 1
 
 
 def _softmax(bars, warp, tiles, meet):
-    """A softmax warp; the first one issues the products (which complete at once)."""
-    for n in range(tiles):
+    """A softmax warp; the first one issues the products (which complete at once).  A window is two
+    products beside O, which every warp reads."""
+    n_pv = n_p = n_t = 0
+    for n, windows in enumerate(tiles):
         yield "K", n
         if meet:
             bars["ready"].arrive()
         if warp == 0:
             if meet:
                 yield "ready", n
-            if n > 0:
-                yield "O", n - 1
+            if n_pv > 0:
+                yield "O", n_pv - 1
             bars["S"].arrive()
         yield "S", n
-        bars["P"].arrive()
-        if warp == 0:
-            yield "V", n
-            yield "P", n
-            bars["O"].arrive()
-    yield "O", tiles - 1
+        for _ in range(max(1, windows)):
+            for half in range(2 if windows else 1):
+                bars["P"].arrive()
+                if warp == 0:
+                    yield "V", n_pv
+                    yield "P", n_p
+                    if windows:
+                        bars["T"].arrive()
+                    if half == 1 or not windows:
+                        bars["O"].arrive()
+                n_p += 1
+                if windows:
+                    yield "T", n_t
+                    n_t += 1
+            n_pv += 1
+    yield "O", n_pv - 1
 
 
-def _run(seed, *, meet, tiles=5):
+def _run(seed, *, meet):
     rng = random.Random(seed)
-    bars = {name: Barrier(1 if name in "SO" else 4) for name in ("K", "V", "P", "S", "O", "ready")}
+    tiles = [rng.choice([0, 0, 0, 1, 3]) for _ in range(5)]
+    bars = {name: Barrier(1 if name in "STO" else 4) for name in ("K", "V", "P", "S", "T", "O", "ready")}
     roles = [_operands(bars, tiles) for _ in range(4)] + [_softmax(bars, w, tiles, meet) for w in range(4)]
     speed = [rng.choice([1, 1, 100]) for _ in roles]
     waits = {i: next(r) for i, r in enumerate(roles)}
-    for _ in range(20000):
-        i = rng.choices(list(waits), [speed[i] for i in waits])[0]
-        name, n = waits[i]
-        if bars[name].passes(n):
-            try:
-                waits[i] = next(roles[i])
-            except StopIteration:
-                del waits[i]
-                if not waits:
-                    return
-    raise AssertionError(f"still waiting: {waits}")
+    while waits:
+        able = [i for i, (name, n) in waits.items() if bars[name].passes(n)]
+        assert able, f"nobody can go on: {waits}"
+        i = rng.choices(able, [speed[i] for i in able])[0]
+        try:
+            waits[i] = next(roles[i])
+        except StopIteration:
+            del waits[i]
 
 
 def test_no_wait_misses_its_phase():
