@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
         const int x = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
         const int up = amax > 0.f && x < 128 ? min(14 - x, 126) : 0;
         const float f = a.scale > 0.f ? pow2f(up) : a.scale < 0.f ? -pow2f(up) : 0.f;
-        const float unit = pow2f(max(-up, -126)) * nat;
+        const float unit = fmaxf(pow2f(max(-up, -126)) * nat, kMinFloat);
 #pragma unroll
         for (int k = 0; k < C::kC; ++k) {
           const uint32_t w[4] = {raw[z][k].x, raw[z][k].y, raw[z][k].z, raw[z][k].w};

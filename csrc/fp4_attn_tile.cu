@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         const int x = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
         const int up = amax > 0.f && x < 128 ? min(14 - x, 126) : 0;  // to fp16's top
         const float f = a.scale > 0.f ? pow2f(up) : a.scale < 0.f ? -pow2f(up) : 0.f;
-        factor = pow2f(max(-up, -126)) * nat;
+        factor = fmaxf(pow2f(max(-up, -126)) * nat, kMinFloat);
 #pragma unroll 4
         for (int k = 0; k < D / 8; ++k) {
           const uint4 raw = *reinterpret_cast<const uint4*>(from + 8 * k);

@@ -221,6 +221,15 @@ def test_values_at_the_type_s_end_reach_only_the_rows_that_see_them(cuda, room):
         _check(cuda, k, v, q, room=room, window=52, extra=2.0 ** -110)
 
 
+@BOTH
+def test_scores_of_the_smallest_factors(cuda, room):
+    """Queries and a scale whose product fp32 does not hold: scores of zero, masks still masks."""
+    gen = torch.Generator().manual_seed(14)
+    for d in (64, 128):
+        q = (2.0 ** -120 * _rand(gen, 1, 8, 9, d)).bfloat16()
+        _check(cuda, _rand(gen, 150, 1, d), _rand(gen, 150, 1, d), q, room=room, scale=2.0 ** -40, window=40)
+
+
 def test_tiles_beside_other_work(cuda):
     """The many-row kernel shares the GPU with other streams' kernels: warps are held up, results are not."""
     from saint_llm_b200.ops.fp4_kv import fp4_kv_attention
