@@ -14,8 +14,9 @@
 //   query rows as the 8 columns: with one to sixteen rows a 128-row tcgen05 tile would be 7/8
 //   empty.  Codes become fp16 pairs with cvt.e2m1x2, exact.
 // * K and V scales are powers of two, applied to the fp16 pairs: exact while the exponent is in
-//   [-14, 13].  A tile with scales outside takes other exponents for K (28 from its own largest
-//   down) and runs its V product once per window of 28 exponents, each added to the sums in fp32.
+//   [-14, 13].  A tile with scales outside takes other exponents for K (28 from each key's own
+//   largest down, so that no key's size touches another's score) and runs its V product once per window of
+//   28 exponents, each added to the sums in fp32.
 // * q is scaled by a power of two per row to the top of fp16's range (bf16 keeps its 8 bits, what
 //   falls below 2^-38 of the row's largest is lost).  p is held times 2^15: fp16's 11 bits for
 //   weights down to 2^-29 of the largest.  A row's maximum is left as it is while the new one is at
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
         const uint32_t low = ((k16 - 0x01010101u) & (v16 - 0x01010101u) & 0x80808080u) ^ 0x80808080u;
         const bool inner = halves == 3u && key0 >= first && key0 + kTile <= last;  // every row was written
         bool plain = true, vnan = false;
-        int kbias = 112, vbias = 112, vhi = 0;
+        int kbias = 112, vbias = 112, vhi = 0;  // kbias: of key key0 + lane
         uint32_t ksc[4], vsc[2][2];
         const int pair_at = (lane & ~7) | ((lane & 3) * 2) | ((lane >> 2) & 1);  // keys c and c + 4 side by side
         auto put_v_scales = [&](int bias, int most) {  // of the blocks whose byte is `most` or less
@@ -329,7 +330,6 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           scale_range(vw, C::kC, vlo, vhi, vnan);
           plain = __all_sync(0xffffffffu, min(klo, vlo) > 112 && max(khi, vhi) <= 140 && !knan && !vnan);  // but for zero blocks
           if (!plain) {
-            khi = __reduce_max_sync(0xffffffffu, khi);
             vhi = __reduce_max_sync(0xffffffffu, vhi);
             kbias = max(khi - 28, kLeastBias);
             vbias = max(vhi - 28, kLeastBias);
@@ -393,13 +393,6 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
         for (int z = 0; z < NT; ++z)
 #pragma unroll
           for (int n = 0; n < 2; ++n) f[z][n] = factor[z][n];
-        if (!plain) {
-          const float km = pow2f(kbias - 112);
-#pragma unroll
-          for (int z = 0; z < NT; ++z)
-#pragma unroll
-            for (int n = 0; n < 2; ++n) f[z][n] = fmaxf(f[z][n] * km, 1.1754944e-38f);  // 0 would turn the mask's -inf into NaN
-        }
         auto each_score = [&](auto&& change) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
@@ -412,6 +405,13 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
 #pragma unroll
           for (int z = 0; z < NT; ++z) f[z][0] = f[z][1] = 1.f;
         };
+        if (!plain) {
+          float km[4];  // units of the keys 8 j + k_row
+#pragma unroll
+          for (int j = 0; j < 4; ++j) km[j] = pow2f(__shfl_sync(0xffffffffu, kbias, 8 * j + k_row) - 112);
+          each_score([&](float v, int j, int z, int p) { return v * fminf(f[z][p & 1] * km[2 * j + (p >> 1)], kMaxFloat); });
+          unit_factors();
+        }
         if (a.softcap > 0.f) {
           const float cap = a.softcap * kLog2e, squeeze = 2.f * kLog2e / a.softcap;
           each_score([&](float v, int, int z, int p) {  // tanh x = 1 - 2 / (1 + e^2x)

@@ -16,7 +16,7 @@
 //   cvt.e2m1x2 to fp16, exact, times their scale 2^e, exact for exponents in [-14, 13].  K and V lie
 //   as 64-column 128B-swizzled atoms, V contracted over its rows.
 //
-// A tile with other exponents takes K's from its own largest 28 down, and runs P V once per window
+// A tile with other exponents takes K's from each key's own largest 28 down, and runs P V once per window
 // of 28 exponents, 64 dims at a time into the half of S that P leaves free; the softmax warps add that to
 // O in fp32.
 #include "fp4_work.cuh"
@@ -63,9 +63,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 struct Tile {
   int plain;   // all exponents in [-14, 13] and every page there, O in units of 1
   int large;   // O is held in units of 2^kLargeUnit
-  int kbias;   // K's scales are 2^(byte - kbias - 15)
   int windows; // products P V
   int bias[kWindows];
+  float kunit[kKeys];  // what a key's scores are multiplied by
   uint32_t nan_keys[kKeys];  // bits 0 - 3: blocks of V that are NaN; bit 31: a key whose page id is bad
 };
 
@@ -77,7 +77,7 @@ struct Cfg {
   static constexpr int kRowsAtOnce = 32 / kC;       // a warp's rows per pass: lane = (block, row)
   static constexpr int kPasses = 32 / kRowsAtOnce;  // a warp writes 32 rows
   // q, K, V, alignment, barriers and tiles; as much for every D, so that two blocks' TMEM is all an SM is asked for
-  static constexpr int kSmem = 6 * kAtom + 1024 + 2048;
+  static constexpr int kSmem = 6 * kAtom + 1024 + 3072;
 };
 
 // The largest v over the four operand warps.
@@ -89,8 +89,9 @@ __device__ __forceinline__ int most_of(int v, int* red, int part, int lane) {
   return max(max(red[0], red[1]), max(red[2], red[3]));
 }
 
-// A tile with exponents outside [-14, 13], NaN blocks or missing keys: K's bias, V's windows and the
-// keys' marks, from the scale bytes (one per pass) of all operand threads.  Returns kbias, and the windows with
+// A tile with exponents outside [-14, 13], NaN blocks or missing keys: the keys' units and
+// marks and V's windows, from the scale bytes (one per pass) of all operand threads.  Returns the biases of
+// this thread's keys (K's scales are 2^(byte - bias - 15)), 14 more in a byte per pass, and the windows with
 // 256 added for V scales above kLargeByte.
 // Not inlined: its registers would be taken from every tile.
 template <int D>
@@ -98,14 +99,18 @@ __device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uin
                                       int part, int lane) {
   using C = Cfg<D>;
   const int in_row = lane % C::kRowsAtOnce, blk = lane / C::kRowsAtOnce;
-  int khi = 0, vhi = 0;
+  int vhi = 0;
+  uint32_t kbias = 0;
   for (int x = 0; x < C::kPasses; ++x) {
-    if (!((seen >> x) & 1u)) continue;
+    const bool mine = (seen >> x) & 1u;
     const int k = (kbytes >> (8 * x)) & 255u, v = (vbytes >> (8 * x)) & 255u;
-    if (k != 255) khi = max(khi, k);
-    if (v != 255) vhi = max(vhi, v);
+    int khi = mine && k != 255 ? k : 0;
+    for (int o = C::kRowsAtOnce; o < 32; o <<= 1) khi = max(khi, __shfl_xor_sync(0xffffffffu, khi, o));
+    const int bias = max(khi - 28, kLeastBias);
+    kbias |= static_cast<uint32_t>(bias - kLeastBias) << (8 * x);
+    if (blk == 0) tile.kunit[32 * part + C::kRowsAtOnce * x + in_row] = pow2f(bias - 112);
+    if (mine && v != 255) vhi = max(vhi, v);
   }
-  const int kbias = max(most_of(khi, red, part, lane) - 28, kLeastBias);
   vhi = most_of(vhi, red, part, lane);
   int bias = max(vhi - 28, kLeastBias), windows = 1;
   const bool scribe = part == 0 && lane == 0;
@@ -129,7 +134,7 @@ __device__ __noinline__ int2 describe(Tile& tile, int* red, uint32_t kbytes, uin
     if (((seen >> x) & 1u) && ((vbytes >> (8 * x)) & 255u) == 255u) atomicOr(tile.nan_keys + row, 1u << blk);
     if ((lost >> x) & 1u) atomicOr(tile.nan_keys + row, 0x80000000u);
   }
-  return make_int2(kbias, windows + (vhi > kLargeByte ? 256 : 0));
+  return make_int2(static_cast<int>(kbias), windows + (vhi > kLargeByte ? 256 : 0));
 }
 
 // kReady: every softmax warp has seen kKFull of the tile.  Without it warp 0 and the operand warps could
@@ -293,7 +298,8 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           break;
         }
         const bool plain = word == 0 && !large;
-        int kbias = 112, windows = 1;
+        uint32_t kbias = (112u - kLeastBias) * 0x01010101u;
+        int windows = 1;
         const bool scribe = part == 0 && lane == 0;
         if (!plain) {
           uint32_t kbytes = 0, vbytes = 0;
@@ -303,19 +309,18 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
             vbytes |= static_cast<uint32_t>(vraw[x]) << (8 * x);
           }
           const int2 found = describe<D>(tile, red, kbytes, vbytes, seen, lost, part, lane);
-          kbias = found.x;
+          kbias = static_cast<uint32_t>(found.x);
           windows = found.y & 255;
           large = large || found.y >= 256;
         }
         if (scribe) {
           tile.plain = plain;
           tile.large = large;
-          tile.kbias = kbias;
           tile.windows = windows;
         }
         write(0, [&](int x) {
           const int k = static_cast<int>(kraw[x]);
-          return !((seen >> x) & 1u) ? 0u : k == 255 ? 0x7e00u : scale_bits(k, kbias);
+          return !((seen >> x) & 1u) ? 0u : k == 255 ? 0x7e00u : scale_bits(k, static_cast<int>((kbias >> (8 * x)) & 255u) + kLeastBias);
         });
         load_codes(a.R * (D / 2));
         fence_proxy_async_smem();
@@ -421,13 +426,13 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         tc_fence_after();
         const Tile& tile = tiles[n_tile & 1];
         const bool plain = tile.plain;
-        float f = factor;
-        if (!plain) f = fmaxf(f * pow2f(tile.kbias - 112), 1.1754944e-38f);  // 0 would turn the mask's -inf into NaN
+        const float f = plain ? factor : 1.f;  // or every key has its own
         const bool masked = key0 < inner_lo || key0 + kKeys > inner_hi, simple = !masked && plain;
         const float cap = a.softcap * kLog2e, squeeze = a.softcap > 0.f ? f * 2.f * kLog2e / a.softcap : 0.f;
         auto capped = [&](float v) { return __fmul_rn(cap, 1.f - __fdividef(2.f, 1.f + ex2(v * squeeze))); };  // tanh x = 1 - 2 / (1 + e^2x)
-        auto visible = [&](uint32_t raw, int j) {  // the raw score of key key0 + j, or -inf
+        auto visible = [&](uint32_t raw, int j) {  // the score of key key0 + j (times f), or -inf
           float v = __uint_as_float(raw);
+          if (!plain) v *= fminf(factor * tile.kunit[j], kMaxFloat);
           if (masked) v = key0 + j >= lo && key0 + j < hi ? v : -INFINITY;
           if (!plain && (tile.nan_keys[j] >> 31)) v = -INFINITY;
           return v;

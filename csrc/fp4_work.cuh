@@ -8,7 +8,8 @@ namespace sv4 {
 namespace fp4 {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kMinFloat = 1.1754944e-38f;  // the least factor of scores: 0 times a mask's -inf would be NaN
+constexpr float kMaxFloat = 3.4028235e38f;   // factors of scores stay finite and above zero: 0 times
+constexpr float kMinFloat = 1.1754944e-38f;  // infinity (a mask's, too) would be NaN
 
 // Four bytes of two codes each -> four fp16 pairs (low code in the low half).
 __device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t (&o)[4]) {

@@ -222,6 +222,23 @@ def test_values_at_the_type_s_end_reach_only_the_rows_that_see_them(cuda, room):
 
 
 @BOTH
+def test_a_key_s_size_does_not_touch_the_others_scores(cuda, room):
+    """Outliers among the keys: far below every other score, or out of a row's window."""
+    gen = torch.Generator().manual_seed(8)
+    for d in (64, 128):
+        for up in (30, 60, 90):
+            q, k, v = _rand(gen, 1, 8, 9, d).abs(), _rand(gen, 300, 1, d), _rand(gen, 300, 1, d)
+            k[[3, 150, 260]] = -k[[3, 150, 260]].abs() * 2.0 ** up
+            _check(cuda, k, v, (0.3 * q).bfloat16(), room=room)
+            k = _rand(gen, 300, 1, d)
+            k[241:246] *= 2.0 ** up
+            _check(cuda, k, v, (0.3 * q[:, :, 5:]).bfloat16(), room=room, window=50)  # rows 296 - 299 see 247 and up
+            k *= 2.0 ** -30
+            k[241:246] *= 2.0 ** 30
+            _check(cuda, k, v, (2.0 ** 28 * q).bfloat16(), room=room, window=52)
+
+
+@BOTH
 def test_scores_of_the_smallest_factors(cuda, room):
     """Queries and a scale whose product fp32 does not hold: scores of zero, masks still masks."""
     gen = torch.Generator().manual_seed(14)
