@@ -413,10 +413,13 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           unit_factors();
         }
         if (a.softcap > 0.f) {
-          const float cap = a.softcap * kLog2e, squeeze = 2.f * kLog2e / a.softcap;
-          each_score([&](float v, int, int z, int p) {  // tanh x = 1 - 2 / (1 + e^2x)
-            return cap * (1.f - __fdividef(2.f, 1.f + ex2(v * f[z][p & 1] * squeeze)));
-          });
+          Cap cap[NT][2];
+#pragma unroll
+          for (int z = 0; z < NT; ++z)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) cap[z][n] = Cap(a.softcap, f[z][n]);
+          if (a.softcap <= kRoundCap) each_score([&](float v, int, int z, int p) { return cap[z][p & 1].round(v); });
+          else each_score([&](float v, int, int z, int p) { return cap[z][p & 1].exact(v); });
           unit_factors();
         }
         if (halves != 3u || key0 < inner_lo || key0 + kTile > inner_hi) {  // some row does not see some key

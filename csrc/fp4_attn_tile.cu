@@ -428,8 +428,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         const bool plain = tile.plain;
         const float f = plain ? factor : 1.f;  // or every key has its own
         const bool masked = key0 < inner_lo || key0 + kKeys > inner_hi, simple = !masked && plain;
-        const float cap = a.softcap * kLog2e, squeeze = a.softcap > 0.f ? f * 2.f * kLog2e / a.softcap : 0.f;
-        auto capped = [&](float v) { return __fmul_rn(cap, 1.f - __fdividef(2.f, 1.f + ex2(v * squeeze))); };  // tanh x = 1 - 2 / (1 + e^2x)
+        const Cap cap = a.softcap > 0.f ? Cap(a.softcap, f) : Cap();
         auto visible = [&](uint32_t raw, int j) {  // the score of key key0 + j (times f), or -inf
           float v = __uint_as_float(raw);
           if (!plain) v *= fminf(factor * tile.kunit[j], kMaxFloat);
@@ -460,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
             for (int j = 0; j < 32; ++j) most = fmaxf(most, visible(r[j], c * 32 + j));
           }
         }
-        if (a.softcap > 0.f) most = most == -INFINITY ? most : capped(most);  // tanh keeps the order
+        if (a.softcap > 0.f) most = most == -INFINITY ? most : cap.exact(most);  // tanh keeps the order
         else most = __fmul_rn(most, f);
         const float next = most > m + lag_of(most) ? most : m;
         out_of_range = out_of_range || (next != -INFINITY && fabsf(next) > kCoarse);
@@ -497,10 +496,10 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
             }
           };
           if (a.softcap > 0.f) {
-            if (fine) weigh([&](int j) { return capped(__uint_as_float(r[j])) + d0; });
+            if (fine && a.softcap <= kRoundCap) weigh([&](int j) { return cap.round(__uint_as_float(r[j])) + d0; });
             else weigh([&](int j) {
               const float v = visible(r[j], c * 32 + j);
-              return v == -INFINITY ? v : below_maximum(capped(v));
+              return v == -INFINITY ? v : below_maximum(cap.exact(v));
             });
           } else if (fine) {
             weigh([&](int j) { return fmaf(__uint_as_float(r[j]), f, d0); });

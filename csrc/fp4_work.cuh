@@ -40,6 +40,27 @@ __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_ca
 // 2^(a - b) for a <= b, both possibly -inf
 __device__ __forceinline__ float shrink(float a, float b) { return a == b ? 1.f : ex2(a - b); }
 
+// c tanh(s / c) in log2 units, s = v f (natural units).  1 - 2 / (1 + e^2x) has an error of some 2^-21 whatever its size
+// (two approximations and what the 1 leaves of them), which c repeats: 3e-5 at kRoundCap.  Above that, and
+// where it costs little, x below 1/4 takes the series of tanh, whose next term is 2^-26 of it.
+constexpr float kRoundCap = 64.f;
+struct Cap {
+  float size, twice, once;
+  __device__ __forceinline__ Cap() {}
+  __device__ __forceinline__ Cap(float c, float f) {
+    size = fminf(c * kLog2e, kMaxFloat);
+    once = fminf(f * fminf(1.f / c, kMaxFloat), kMaxFloat);
+    twice = fminf(once * (2.f * kLog2e), kMaxFloat);
+  }
+  __device__ __forceinline__ float tanh_of(float v) const { return 1.f - __fdividef(2.f, 1.f + ex2(v * twice)); }
+  __device__ __forceinline__ float round(float v) const { return __fmul_rn(size, tanh_of(v)); }
+  __device__ __forceinline__ float exact(float v) const {
+    const float x = v * once, y = x * x;
+    const float series = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+    return __fmul_rn(size, fabsf(x) < 0.25f ? series : tanh_of(v));
+  }
+};
+
 // Maxima above this are spaced by 2^-7 and more.  How far a row's maximum may lag behind the scores: fp16
 // holds p (times 2^15) up to 2^15.99, and 0.9 is 0.9 only where fp32 is fine enough.
 constexpr float kCoarse = 65536.f;

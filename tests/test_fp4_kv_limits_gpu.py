@@ -247,6 +247,25 @@ def test_scores_of_the_smallest_factors(cuda, room):
         _check(cuda, _rand(gen, 150, 1, d), _rand(gen, 150, 1, d), q, room=room, scale=2.0 ** -40, window=40)
 
 
+@BOTH
+@pytest.mark.parametrize("softcap", [40.0, 70.0, 3e3, 1e5, 1e7, 1e30])
+def test_large_softcaps(cuda, room, softcap):
+    gen = torch.Generator().manual_seed(9)
+    for n in (3, 40, 200):
+        for size in (0.05, 0.5, 3.0):
+            q = (size * _rand(gen, 1, 12, 9 if n > 9 else 3, 64)).half()
+            _check(cuda, _rand(gen, n, 1, 64), _rand(gen, n, 1, 64), q, room=room, softcap=softcap, scale=0.3)
+
+
+@BOTH
+def test_softcap_of_the_smallest_size(cuda, room):
+    """Scores that a softcap of 1e-40 leaves: all the same."""
+    gen = torch.Generator().manual_seed(10)
+    q = _rand(gen, 1, 12, 9, 64).bfloat16()
+    q[:, ::2] = 0.0
+    _check(cuda, _rand(gen, 60, 1, 64), _rand(gen, 60, 1, 64), q, room=room, softcap=1e-40)
+
+
 def test_tiles_beside_other_work(cuda):
     """The many-row kernel shares the GPU with other streams' kernels: warps are held up, results are not."""
     from saint_llm_b200.ops.fp4_kv import fp4_kv_attention
