@@ -30,6 +30,7 @@ from saint_llm_b200.models.attention.common import rope_tables
 from saint_llm_b200.models.mhc import MHC
 from saint_llm_b200.ops import pages as page_ops
 from saint_llm_b200.ops.fp4_kv import fp4_kv_attention, fp4_kv_read, fp4_kv_slab_bytes, fp4_kv_write
+from saint_llm_b200.ops.gemm import check_errors
 
 
 class Fp4KVCache:
@@ -112,6 +113,20 @@ def _check_model(model: nn.Module) -> None:
         raise ValueError("the 4-bit cache does not support prepended sink tokens")
 
 
+def _check_cache(model: nn.Module, cache: Fp4KVCache, n: int, length: int, device: torch.device) -> None:
+    d = model.cfg.attention.head_dim  # type: ignore[attr-defined]
+    if cache.pool.shape[1] < len(model.blocks) or cache.pool.shape[2] != 1 or cache.head_dim != d:  # type: ignore[attr-defined]
+        raise ValueError(f"the cache holds {cache.pool.shape[1]} layers of {cache.pool.shape[2]} heads of {cache.head_dim}, the "
+                         f"model has {len(model.blocks)} of 1 head of {d}")  # type: ignore[attr-defined]
+    if cache.pool.device != device:
+        raise ValueError(f"the cache is on {cache.pool.device}, the prompts are on {device}")
+    if n > cache.table.shape[0] or length > cache.table.shape[1] * cache.page_rows:
+        raise ValueError(f"{n} sequences of {length} rows: the cache has {cache.table.shape[0]} sequences of up to "
+                         f"{cache.table.shape[1] * cache.page_rows}")
+    if bool(cache.lengths[:n].any()):
+        raise ValueError(f"sequences 0 .. {n - 1} of the cache must be empty")
+
+
 def _last_logits(model: nn.Module, cache: Fp4KVCache, ids: Tensor, seqs: Tensor, start: int) -> Tensor:
     """(n, V) logits after the tokens ``ids`` (n, T) of sequences ``seqs``, which stand at ``start``."""
     cfg = model.cfg  # type: ignore[attr-defined]
@@ -125,7 +140,7 @@ def _last_logits(model: nn.Module, cache: Fp4KVCache, ids: Tensor, seqs: Tensor,
         q = a._queries(inner, cos, sin)
         cache.write(layer, *a._sw_kv(inner, cos, sin), slots)
         if q.is_cuda and q.dtype == torch.float32:
-            q = q.bfloat16()
+            q = q.bfloat16()  # the kernels take 16 bits; bf16 keeps fp32's range, for outputs as large as V is
         out = cache.attend(layer, q, seqs, window=a.attn_cfg.sliding_window_size, sink=a.sink_logit,
                            softcap=a.attn_cfg.logit_softcap)
         x = blk.attn_mhc.combine(x, a.output(out.to(x.dtype)), b_l, c_l)
@@ -145,36 +160,47 @@ def fp4_beam_search(model: nn.Module, prompt_ids: Tensor, *, beams: int, max_new
     """Beam search of prompts (B, T) on a 4-bit cache: the ids (B, beams, T + max_new_tokens) and the
     sums of log-probabilities (B, beams), best first.  Prompts are prefilled once, in chunks; the
     beams of a prompt share its pages.  ``cache`` (its sequences 0 .. B * beams - 1 empty) is used
-    and emptied again; by default one of the size needed is made."""
+    and emptied again, whatever happens; by default one of the size needed is made.  A cache that
+    does not fit the model or the request is refused; one whose pool runs out of pages raises
+    ``PoolExhausted`` (on CUDA ``RuntimeError``, after the last step).  On CUDA the attention of an
+    fp32 model takes its queries and gives its outputs in bf16."""
     _check_model(model)
     b, t = prompt_ids.shape
     n = b * beams
-    if beams <= 0 or max_new_tokens <= 0 or t == 0:
-        raise ValueError("beams, max_new_tokens and the prompt's length must be positive")
+    if beams <= 0 or max_new_tokens <= 0 or t == 0 or prefill_chunk <= 0:
+        raise ValueError("beams, max_new_tokens, prefill_chunk and the prompt's length must be positive")
     cfg, dev = model.cfg, prompt_ids.device  # type: ignore[attr-defined]
+    if beams > cfg.vocab_size:
+        raise ValueError(f"{beams} beams of {cfg.vocab_size} tokens")
     total = t + max_new_tokens
     if cache is None:
         # the prompts, and for every beam its own pages from the prompt's last one on, twice during a fork
         own = -(-total // page_rows) - t // page_rows + 1
         cache = Fp4KVCache(len(model.blocks), b * (-(-t // page_rows)) + 2 * n * own, max_seqs=n,  # type: ignore[attr-defined]
                            max_len=total, head_dim=cfg.attention.head_dim, page_rows=page_rows, device=dev)
+    else:
+        _check_cache(model, cache, n, total - 1, dev)  # the last tokens are not fed
     every = torch.arange(n, dtype=torch.int32, device=dev)
     first = every[::beams].contiguous()
-    logits = None
-    for c in range(0, t, prefill_chunk):
-        logits = _last_logits(model, cache, prompt_ids[:, c:c + prefill_chunk], first, c)
-    cache.fork(first.repeat_interleave(beams), every)
-    logp = torch.log_softmax(logits, -1)
-    scores, tokens = logp.topk(beams, -1)  # (B, beams)
-    ids = torch.cat([prompt_ids.repeat_interleave(beams, 0), tokens.reshape(n, 1)], 1)
-    for step in range(1, max_new_tokens):
-        logp = torch.log_softmax(_last_logits(model, cache, ids[:, -1:], every, t + step - 1), -1)
-        scores, pick = (scores.unsqueeze(-1) + logp.view(b, beams, -1)).flatten(1).topk(beams, -1)
-        parents = (pick // logp.shape[-1] + torch.arange(b, device=dev).unsqueeze(1) * beams).reshape(-1)
-        ids = torch.cat([ids[parents], (pick % logp.shape[-1]).reshape(n, 1)], 1)
-        if step + 1 < max_new_tokens:  # the last tokens are not fed again
-            cache.fork(parents, every)
-    cache.free(every)
+    try:
+        logits = None
+        for c in range(0, t, prefill_chunk):
+            logits = _last_logits(model, cache, prompt_ids[:, c:c + prefill_chunk], first, c)
+        cache.fork(first.repeat_interleave(beams), every)
+        logp = torch.log_softmax(logits, -1)
+        scores, tokens = logp.topk(beams, -1)  # (B, beams)
+        ids = torch.cat([prompt_ids.repeat_interleave(beams, 0), tokens.reshape(n, 1)], 1)
+        for step in range(1, max_new_tokens):
+            logp = torch.log_softmax(_last_logits(model, cache, ids[:, -1:], every, t + step - 1), -1)
+            scores, pick = (scores.unsqueeze(-1) + logp.view(b, beams, -1)).flatten(1).topk(beams, -1)
+            parents = (pick // logp.shape[-1] + torch.arange(b, device=dev).unsqueeze(1) * beams).reshape(-1)
+            ids = torch.cat([ids[parents], (pick % logp.shape[-1]).reshape(n, 1)], 1)
+            if step + 1 < max_new_tokens:  # the last tokens are not fed again
+                cache.fork(parents, every)
+    finally:
+        cache.free(every)
+    if dev.type == "cuda":
+        check_errors(dev)  # no free page, an index out of range: the tokens would be made without some rows
     return ids.view(b, beams, -1), scores
 
 

@@ -1,5 +1,5 @@
 """Beam search on the 4-bit cache against the model itself: with the cache's rows kept in fp32, what it
-scores is what the model scores; a step's fork matters."""
+scores is what the model scores; a step's fork matters; a cache that does not fit is refused."""
 
 import math
 
@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from saint_llm_b200.infer.fp4_cache import Fp4KVCache, _last_logits, fp4_beam_search
+from saint_llm_b200.infer.paged_kv import PoolExhausted
 
 
 class ExactCache(Fp4KVCache):
@@ -124,6 +125,47 @@ def test_four_bits_score_near_the_model():
         got = _last_logits(model, cache, ids, torch.arange(2, dtype=torch.int32), 0)
         want = model(ids)["logits"][:, -1]
     assert float((got - want).norm() / want.norm()) < 0.25
+
+
+def test_a_cache_that_does_not_fit_is_refused():
+    model, prompt = _model(), _prompt(1, 9)
+    search = lambda **kw: fp4_beam_search(model, prompt, beams=4, max_new_tokens=9, **kw)  # noqa: E731
+    kw = {"max_seqs": 4, "max_len": 40, "head_dim": 32, "page_rows": 16}
+    for wrong in (Fp4KVCache(1, 60, **kw), Fp4KVCache(2, 60, **{**kw, "max_seqs": 3}), Fp4KVCache(2, 60, **{**kw, "max_len": 16}),
+                  Fp4KVCache(2, 60, **{**kw, "head_dim": 64}), Fp4KVCache(2, 60, kv_heads=2, **kw)):
+        with pytest.raises(ValueError):
+            search(cache=wrong)
+        assert not wrong.refcount.any()
+    used = Fp4KVCache(2, 60, **kw)
+    used.reserve([2], 3)
+    with pytest.raises(ValueError, match="empty"):
+        search(cache=used)
+    with pytest.raises(ValueError):
+        fp4_beam_search(model, prompt, beams=10 ** 6, max_new_tokens=2)
+    with pytest.raises(ValueError):
+        fp4_beam_search(model, prompt, beams=2, max_new_tokens=2, prefill_chunk=0)
+    ok = Fp4KVCache(2, 60, **{**kw, "max_len": 17})  # the last token is never fed: 17 rows
+    search(cache=ok)
+
+
+def test_a_search_that_fails_leaves_the_cache_empty():
+    model, prompt = _model(), _prompt(1, 9)
+    cache = Fp4KVCache(2, 3, max_seqs=4, max_len=40, head_dim=32, page_rows=16)
+    with pytest.raises(PoolExhausted):
+        fp4_beam_search(model, prompt, beams=4, max_new_tokens=9, cache=cache)
+    assert not cache.refcount.any() and not cache.lengths.any() and bool((cache.table == -1).all())
+
+
+@pytest.mark.gpu
+def test_a_search_without_pages_raises_on_the_gpu(cuda):
+    from saint_llm_b200.ops.gemm import check_errors
+
+    model, prompt = _model(cuda, torch.bfloat16), _prompt(1, 9).to(cuda)
+    cache = Fp4KVCache(2, 3, max_seqs=4, max_len=40, head_dim=32, page_rows=16, device=cuda)
+    with pytest.raises(RuntimeError, match="no free page"):
+        fp4_beam_search(model, prompt, beams=4, max_new_tokens=9, cache=cache)
+    check_errors(cuda)
+    assert not cache.refcount.any() and not cache.lengths.any() and bool((cache.table == -1).all())
 
 
 @pytest.mark.gpu
