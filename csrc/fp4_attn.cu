@@ -430,6 +430,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
           });
         }
         float next[NT][2];
+        const float lag = out_of_range ? 0.f : kLag;
         bool moved = false;
         float most = 0.f;
 #pragma unroll
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
             const float now = __fmul_rn(x, f[z][n]);
-            next[z][n] = now > m[z][n] + lag_of(now) ? now : m[z][n];
+            next[z][n] = now > m[z][n] + lag ? now : m[z][n];
             moved = moved || next[z][n] != m[z][n];
             most = fmaxf(most, next[z][n] == -INFINITY ? 0.f : fabsf(next[z][n]));
           }
@@ -463,6 +464,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
             m[z][1] = next[z][1];
           }
         }
+        float d[NT][2];
+#pragma unroll
+        for (int z = 0; z < NT; ++z)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) d[z][n] = m[z][n] == -INFINITY ? 0.f : 15.f - m[z][n];
         if (out_of_range) {
           // The maximum is taken off first, from scores that were rounded as it was: 15 - m below would be rounded
           // to the spacing of m, 16 - m from 2^24 on, and p would pass fp16's end.
@@ -470,18 +476,18 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NT>::kBlocks) fp4_attn_row
             return __fsub_rn(__fmul_rn(v, f[z][p & 1]), m[z][p & 1] == -INFINITY ? 0.f : m[z][p & 1]);
           });
           unit_factors();
+#pragma unroll
+          for (int z = 0; z < NT; ++z) d[z][0] = d[z][1] = 15.f;
         }
         // p times 2^15 (a row without a key so far keeps p = 0), as the B operand of the next product
         uint32_t p[2][NT][2];
 #pragma unroll
         for (int z = 0; z < NT; ++z) {
-          const float d0 = out_of_range ? 15.f : m[z][0] == -INFINITY ? 0.f : 15.f - m[z][0];
-          const float d1 = out_of_range ? 15.f : m[z][1] == -INFINITY ? 0.f : 15.f - m[z][1];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
-              p[j][z][x] = transpose8(pack_half2(ex2(fmaf(s[j][z][2 * x], f[z][0], d0)), ex2(fmaf(s[j][z][2 * x + 1], f[z][1], d1))));
+              p[j][z][x] = transpose8(pack_half2(ex2(fmaf(s[j][z][2 * x], f[z][0], d[z][0])), ex2(fmaf(s[j][z][2 * x + 1], f[z][1], d[z][1]))));
           }
           // the rounded weights' sums, as a product with ones
 #pragma unroll

@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
         }
         if (a.softcap > 0.f) most = most == -INFINITY ? most : cap.exact(most);  // tanh keeps the order
         else most = __fmul_rn(most, f);
-        const float next = most > m + lag_of(most) ? most : m;
+        const float next = most > m + (out_of_range ? 0.f : kLag) ? most : m;
         out_of_range = out_of_range || (next != -INFINITY && fabsf(next) > kCoarse);
         if (t > 0 && __any_sync(0xffffffffu, next != m)) {
           const float keep = shrink(m, next);

@@ -63,8 +63,7 @@ struct Cap {
 
 // Maxima above this are spaced by 2^-7 and more.  How far a row's maximum may lag behind the scores: fp16
 // holds p (times 2^15) up to 2^15.99, and 0.9 is 0.9 only where fp32 is fine enough.
-constexpr float kCoarse = 65536.f;
-__device__ __forceinline__ float lag_of(float score) { return fabsf(score) > kCoarse ? 0.f : 0.9f; }
+constexpr float kCoarse = 65536.f, kLag = 0.9f;
 
 __device__ __forceinline__ float2 two_floats(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
 __device__ __forceinline__ float2 two_floats(uint32_t w, __nv_bfloat16) {
