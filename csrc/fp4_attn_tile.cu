@@ -506,6 +506,8 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_attn_tile_kernel(const Fp4Att
           } else {
             weigh([&](int j) { return below_maximum(__fmul_rn(visible(r[j], c * 32 + j), f)); });
           }
+          // before rounding to fp16: roundings of 2^-12 either way, which the outputs' own hide (the other kernel sums
+          // the rounded ones, for there a product with ones is the cheaper sum)
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_st16(ts + c * 16, h);  // over columns of S that have been read
         }

@@ -14,6 +14,10 @@ keeps its addresses, so a step captured in a CUDA graph follows forks and compac
 replays; what went wrong on the device -- no free page, an index out of range -- is raised by
 ``ops.gemm.check_errors``.
 
+Lengths grow by ``reserve`` and are replaced by ``fork`` and ``free``: single tokens are not taken back
+(a smaller number written into ``lengths`` would leave their pages behind), and pages that lie
+behind every window are kept.
+
 ``fp4_beam_search`` decodes sliding-window models with it: one prefill per prompt, a fork to all
 beams, then a reserve, one write and attention per layer, and a fork per step.
 """

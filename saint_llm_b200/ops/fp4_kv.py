@@ -178,7 +178,12 @@ def fp4_kv_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, *
     pages' K / V heads; query head h reads K / V head ``h // (H / kv_heads)``.  ``sink`` (H,): a
     logit that joins the denominator; ``softcap``: scores become ``c tanh(s / c)``; ``scale``:
     default 1 / sqrt(head_dim).  A query without a key gives zeros.  Returns q's shape and type.
-    No value of ``lengths`` is read on the host, so the call can be captured in a CUDA graph."""
+    No value of ``lengths`` is read on the host, so the call can be captured in a CUDA graph.
+
+    On CUDA weights are rounded to fp16 (11 bits down to 2^-29 of a row's largest, none below 2^-39);
+    a score loses what is 28 binades under its key's largest block of K or 38 under its row's largest
+    q; beside values of 2^79 and more, outputs lose what is below 2^-110.  Sums and the softmax's
+    statistics are fp32."""
     one = q.dim() == 3
     if one:
         q = q.unsqueeze(2)
