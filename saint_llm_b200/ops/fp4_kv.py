@@ -162,8 +162,12 @@ def fp4_kv_attention_reference(q: Tensor, pages: Tensor, table: Tensor, lengths:
     total = p.sum(-1, keepdim=True)
     if sink is not None:
         total = total + torch.exp(sink.to(wide).view(1, hk, h // hk, 1, 1) - m)
-    out = torch.einsum("bkgtn,bkgnd->bkgtd", p, v.expand(b, hk, h // hk, n, d))
+    # a block that reads as NaN reaches the queries that see its key, and no others (0 times NaN would)
+    bad = v.isnan()
+    out = torch.einsum("bkgtn,bkgnd->bkgtd", p, torch.where(bad, 0.0, v).expand(b, hk, h // hk, n, d))
+    hit = torch.einsum("btn,bknd->bktd", seen.expand(b, t, n).to(wide), bad.squeeze(2).to(wide)) > 0
     out = out / torch.where(total == 0, torch.ones_like(total), total)
+    out = torch.where(hit.unsqueeze(2), float("nan"), out)
     return out.reshape(b, h, t, d).to(q.dtype)
 
 
