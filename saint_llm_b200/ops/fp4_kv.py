@@ -16,7 +16,7 @@ zero becomes +0.  A block that holds a NaN or an infinity reads back as NaN.
 
 CPU tensors (and ``backend.eager_mode()``) take the definitions below; CUDA tensors run
 ``csrc/fp4_kv.cu``.  An index outside the pool or the table is recorded on the device and raised
-by ``ops.gemm.check_errors``; the row it names is skipped.
+by ``ops.gemm.check_errors``; the row it names is skipped.  The definitions raise ``IndexError``.
 """
 
 from __future__ import annotations
@@ -129,6 +129,18 @@ def fp4_kv_read(pages: Tensor, slots: Tensor, *, head_dim: int,
     return (torch.where(keep, _decode(kc, ks), zero).to(dtype), torch.where(keep, _decode(vc, vs), zero).to(dtype))
 
 
+def _check_table(pages: Tensor, table: Tensor, lengths: Tensor, rows: int, tokens: int, window: int) -> None:
+    """Raises where a key that some query sees is in no page of the pool (host check: CPU tensors)."""
+    room = table.shape[1] * rows
+    if bool((lengths > room).any()):
+        raise IndexError(f"lengths must be at most {room}, the rows of a table row's pages")
+    first = (lengths - tokens + 1 - window).clamp(min=0) if window > 0 else torch.zeros_like(lengths)
+    page = torch.arange(table.shape[1], device=table.device).unsqueeze(0)
+    seen = (page * rows < lengths.unsqueeze(1)) & ((page + 1) * rows > first.unsqueeze(1))
+    if bool((seen & ((table < 0) | (table >= pages.shape[0]))).any()):
+        raise IndexError(f"table ids must be in [0, {pages.shape[0]})")
+
+
 def fp4_kv_attention_reference(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, *, window: int = 0,
                                sink: Tensor | None = None, softcap: float | None = None,
                                scale: float | None = None) -> Tensor:
@@ -137,7 +149,7 @@ def fp4_kv_attention_reference(q: Tensor, pages: Tensor, table: Tensor, lengths:
     rows = fp4_kv_page_rows(pages, d)
     hk = pages.shape[1]
     wide = torch.promote_types(q.dtype, torch.float32)
-    kc, vc, ks, vs = _parts(pages[table.long().clamp(min=0)], rows, d)  # (B, P, heads, rows, ...)
+    kc, vc, ks, vs = _parts(pages[table.long().clamp(0, pages.shape[0] - 1)], rows, d)  # (B, P, heads, rows, ...)
     n = table.shape[1] * rows
     k = _decode(kc, ks).transpose(1, 2).reshape(b, hk, 1, n, d).to(wide)
     v = _decode(vc, vs).transpose(1, 2).reshape(b, hk, 1, n, d).to(wide)
@@ -203,6 +215,7 @@ def fp4_kv_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, *
             raise ValueError("table and lengths must be int32")
         if q.shape[1] % pages.shape[1] or window < 0 or (softcap or 0.0) < 0:
             raise ValueError("H must be a multiple of the K / V heads; window and softcap must not be negative")
+        _check_table(pages, table, lengths, fp4_kv_page_rows(pages, q.shape[3]), q.shape[2], window)
         out = fp4_kv_attention_reference(q, pages, table, lengths, window=window, sink=sink, softcap=softcap,
                                          scale=scale)
     return out.squeeze(2) if one else out

@@ -29,3 +29,24 @@ def test_nan_blocks_reach_only_the_queries_that_see_them(which, hk, value):
         hit = torch.zeros_like(got, dtype=torch.bool)
         hit[:, heads, seen, :64 if which == "k" else 32] = True
         assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], clean[~hit])
+
+
+def test_keys_without_a_page_are_refused():
+    gen = torch.Generator().manual_seed(1)
+    pages = torch.zeros(3, 1, fp4_kv_slab_bytes(16, 64), dtype=torch.uint8)
+    q = torch.randn(2, 4, 2, 64, generator=gen)
+    lengths = torch.tensor([40, 16], dtype=torch.int32)
+    table = torch.tensor([[2, 0, 1], [0, -1, 9]], dtype=torch.int32)  # what no query sees may be anything
+    fp4_kv_attention(q, pages, table, lengths)
+    for row, column, page in ((0, 2, -1), (0, 0, 3), (1, 0, -1)):
+        broken = table.clone()
+        broken[row, column] = page
+        with pytest.raises(IndexError):
+            fp4_kv_attention(q, pages, broken, lengths)
+    broken = table.clone()
+    broken[0, 0] = -1
+    fp4_kv_attention(q, pages, broken, lengths, window=22)  # keys 17 and up
+    with pytest.raises(IndexError):
+        fp4_kv_attention(q, pages, broken, lengths, window=24)
+    with pytest.raises(IndexError):
+        fp4_kv_attention(q, pages, table, torch.tensor([49, 1], dtype=torch.int32))
