@@ -407,7 +407,8 @@ torch::Tensor fp4_kv_attention(torch::Tensor q, torch::Tensor pages, torch::Tens
   const int64_t keys = window > 0 ? std::min<int64_t>(table.size(1) * a.R, window + T) : table.size(1) * a.R;
   const bool many = d >= 64 && pages.size(0) > 0 && many_rows(B * Hk, H / Hk * T, keys);
   const Fp4AttnPlan plan = many ? fp4_attn_tile_plan(a) : fp4_attn_rows_plan(a, static_cast<int>(d));
-  TORCH_CHECK(plan.units < INT32_MAX, "fp4_kv_attention: more than 2^31 tiles of work in one call");
+  TORCH_CHECK(plan.units < INT32_MAX, "fp4_kv_attention: the table has room for more than 2^31 tiles of work (its width counts, not the lengths); "
+              "split the batch");
   a.blocks = plan.blocks;
   const int64_t part_rows = static_cast<int64_t>(plan.blocks) * 2 * plan.rows;
   torch::Tensor parts = uninitialised({part_rows * (d + 2)}, at::kFloat, q);

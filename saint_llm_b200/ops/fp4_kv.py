@@ -194,7 +194,8 @@ def fp4_kv_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, *
     pages' K / V heads; query head h reads K / V head ``h // (H / kv_heads)``.  ``sink`` (H,): a
     logit that joins the denominator; ``softcap``: scores become ``c tanh(s / c)``; ``scale``:
     default 1 / sqrt(head_dim).  A query without a key gives zeros.  Returns q's shape and type.
-    No value of ``lengths`` is read on the host, so the call can be captured in a CUDA graph.
+    No value of ``lengths`` is read on the host, so the call can be captured in a CUDA graph; a table
+    that is wide enough for 2^31 tiles of 32 keys and 8 or 16 query rows is refused.
 
     On CUDA weights are rounded to fp16 (11 bits down to 2^-29 of a row's largest, none below 2^-39);
     a score loses what is 28 binades under its key's largest block of K or 38 under its row's largest

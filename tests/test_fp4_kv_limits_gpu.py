@@ -289,3 +289,16 @@ def test_tiles_beside_other_work(cuda):
     torch.cuda.synchronize()
     check_errors(cuda)
     assert all(torch.equal(o, want) for o in outs)
+
+
+@BOTH
+@pytest.mark.parametrize("low,high", [(-126, 70), (-120, 120), (60, 124)])
+def test_every_window_of_exponents(cuda, room, low, high):
+    """V rows of all sizes in one tile, and queries that pick among them; beside values of 2^79 and up
+    the smallest outputs lose 2^-110."""
+    gen = torch.Generator().manual_seed(15)
+    for d in (64, 128):
+        v = _rand(gen, 260, 1, d) * 2.0 ** torch.randint(low, high + 1, (260, d // 32), generator=gen) \
+            .repeat_interleave(32, -1).view(260, 1, d)
+        q = (8.0 * _rand(gen, 1, 8, 9, d)).bfloat16()
+        _check(cuda, _rand(gen, 260, 1, d), v, q, room=room, window=130, extra=2.0 ** -110 if high > 78 else 0.0)
