@@ -121,10 +121,10 @@ def _operand_loop(meeting, words, warp, fails_at, tiles, agree):
         turn = meeting.turns
         if meeting.arrived == 4:
             meeting.arrived, meeting.turns = 0, meeting.turns + 1
-            meeting.verdict = any(words)
+            meeting.stop = any(words)
         while meeting.turns == turn:
             yield
-        if agree and meeting.verdict:
+        if agree and meeting.stop:
             return
         if fails_at == n:
             alive = False
